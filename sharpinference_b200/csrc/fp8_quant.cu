@@ -1,0 +1,196 @@
+// Quantisation to block-scaled 8-bit values (the definition is in fp8.cuh).
+//
+//   rows     x [M, K] float32 or bfloat16 (rows may lie apart, `rows` may gather them) -> q [M, K] e4m3, scale [blocks, M]:
+//            a scale for 128 neighbours of one row.  A block's scales of all rows lie together, which is how the products
+//            read them (a thread a row).
+//   weight   w [E, N, K] -> q [E, N, K], scale [E, ceil(N / 128), ceil(K / 128)]: a scale for 128 rows by 128 columns.
+//
+// Rows of q are `ldq` bytes apart, a multiple of 16 (what a TMA copy of them needs); the bytes behind K are zeros.
+//
+// Both read their input once, in 16-byte pieces that stay in registers between the maximum and the rounding, and write a
+#include "fp8.cuh"
+
+namespace {
+
+template <typename T> struct Piece;                      // 16 bytes of input
+template <> struct Piece<float> {
+    static constexpr int N = 4;
+    static __device__ __forceinline__ void load(const float* p, float (&v)[4]) {
+        const float4 x = *reinterpret_cast<const float4*>(p);
+        v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+    }
+};
+template <> struct Piece<bf16> {
+    static constexpr int N = 8;
+    static __device__ __forceinline__ void load(const bf16* p, float (&v)[8]) {
+        const uint4 x = *reinterpret_cast<const uint4*>(p);
+        const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            v[2 * i] = __uint_as_float(w[i] << 16);
+            v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        }
+    }
+};
+
+// The elements k .. k + N - 1 of a row of K; zeros behind its end.  VEC: every piece that starts inside the row may be
+// read whole or is cut by the end (16-byte alignment of the row's start is given).
+template <typename T, bool VEC>
+__device__ __forceinline__ void load_piece(const T* row, int k, int K, float (&v)[Piece<T>::N]) {
+    constexpr int N = Piece<T>::N;
+    if (VEC && k + N <= K) {
+        Piece<T>::load(row + k, v);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = k + i < K ? to_float(row[k + i]) : 0.0f;
+    }
+}
+
+template <int N>
+__device__ __forceinline__ uint32_t amax_of(const float (&v)[N]) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) m = max(m, fp8::abs_bits(v[i]));
+    return m;
+}
+
+// The piece in 8 bits at dst (4 or 8 bytes, aligned so); `room`: bytes of the row from there on.
+template <int N>
+__device__ __forceinline__ void store_piece(uint8_t* dst, int room, const float (&v)[N], float inv) {
+    if (room <= 0) return;                               // ldq is a multiple of 16: a piece fits whole or not at all
+    uint32_t w[N / 4];
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i) w[i] = fp8::pack4(v[4 * i] * inv, v[4 * i + 1] * inv, v[4 * i + 2] * inv, v[4 * i + 3] * inv);
+    if constexpr (N == 4) *reinterpret_cast<uint32_t*>(dst) = w[0];
+    else *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
+}
+
+constexpr int ROWS_WARPS = 8, ROWS_EACH = 4;
+
+// A warp takes 512 bytes of each of four neighbouring rows: one block (float32) or two (bfloat16) of each.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(ROWS_WARPS * 32)
+fp8_rows_kernel(const T* x, long long ldx, const int* rows, int M, int K, uint8_t* q, long long ldq, float* scale) {
+    constexpr int N = Piece<T>::N, LANES = fp8::BLOCK / N, SIDE = 32 / LANES;
+    pdl_wait();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int kb = (blockIdx.y * ROWS_WARPS + warp) * SIDE + lane / LANES;
+    const int k = kb * fp8::BLOCK + (lane % LANES) * N;
+    const long long row0 = (long long)blockIdx.x * ROWS_EACH;
+    float v[ROWS_EACH][N];
+#pragma unroll
+    for (int r = 0; r < ROWS_EACH; ++r) {
+        const long long m = min(row0 + r, (long long)M - 1);
+        load_piece<T, VEC>(x + (rows ? rows[m] : m) * ldx, k, K, v[r]);
+    }
+    float s[ROWS_EACH];
+#pragma unroll
+    for (int r = 0; r < ROWS_EACH; ++r) {
+        uint32_t m = amax_of<N>(v[r]);
+#pragma unroll
+        for (int o = LANES / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+        s[r] = fp8::scale_of(m);
+    }
+#pragma unroll
+    for (int r = 0; r < ROWS_EACH; ++r)
+        if (row0 + r < M) store_piece<N>(q + (row0 + r) * ldq + k, (int)(ldq - k), v[r], 1.0f / s[r]);
+    if (lane % LANES == 0 && kb * fp8::BLOCK < K) {
+        float* dst = scale + (long long)kb * M + row0;
+        if (M % 4 == 0) {
+            *reinterpret_cast<float4*>(dst) = make_float4(s[0], s[1], s[2], s[3]);
+        } else {
+#pragma unroll
+            for (int r = 0; r < ROWS_EACH; ++r)
+                if (row0 + r < M) dst[r] = s[r];
+        }
+    }
+}
+
+constexpr int WEIGHT_THREADS = 256;
+
+// A CTA takes a block of 128 x 128.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(WEIGHT_THREADS)
+fp8_weight_kernel(const T* w, int N_, int K, long long ldw, long long group, uint8_t* q, long long ldq, float* scale) {
+    constexpr int N = Piece<T>::N, LANES = fp8::BLOCK / N, SIDE = WEIGHT_THREADS / LANES, EACH = fp8::BLOCK / SIDE;
+    __shared__ uint32_t part[WEIGHT_THREADS / 32];
+    pdl_wait();
+    const int k = blockIdx.x * fp8::BLOCK + (threadIdx.x % LANES) * N;
+    const int n0 = blockIdx.y * fp8::BLOCK + threadIdx.x / LANES;
+    const T* src = w + blockIdx.z * group;
+    float v[EACH][N];
+    uint32_t m = 0;
+#pragma unroll
+    for (int r = 0; r < EACH; ++r) {
+        const int n = n0 + r * SIDE;
+        if (n < N_) {
+            load_piece<T, VEC>(src + n * ldw, k, K, v[r]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) v[r][i] = 0.0f;
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < EACH; ++r) m = max(m, amax_of<N>(v[r]));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = m;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < WEIGHT_THREADS / 32; ++i) m = max(m, part[i]);
+    const float s = fp8::scale_of(m), inv = 1.0f / s;
+    uint8_t* dst = q + ((long long)blockIdx.z * N_) * ldq;
+#pragma unroll
+    for (int r = 0; r < EACH; ++r) {
+        const int n = n0 + r * SIDE;
+        if (n < N_) store_piece<N>(dst + n * ldq + k, (int)(ldq - k), v[r], inv);
+    }
+    if (threadIdx.x == 0) scale[((long long)blockIdx.z * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x] = s;
+}
+
+template <typename T>
+bool vectors(const void* x, long long ld, long long group) {
+    return (reinterpret_cast<uintptr_t>(x) & 15) == 0 && ld * (long long)sizeof(T) % 16 == 0 && group * (long long)sizeof(T) % 16 == 0;
+}
+
+template <typename T>
+int rows_impl(const void* x, long long ldx, const int* rows, int M, int K, void* q, long long ldq, float* scale, cudaStream_t stream) {
+    constexpr int SIDE = 32 / (fp8::BLOCK / Piece<T>::N);
+    const int blocks = (K + fp8::BLOCK - 1) / fp8::BLOCK;
+    const dim3 grid((M + ROWS_EACH - 1) / ROWS_EACH, (blocks + ROWS_WARPS * SIDE - 1) / (ROWS_WARPS * SIDE));
+    if (grid.y > 65535) return SHARPI_BAD_ARGUMENT;
+    const T* src = static_cast<const T*>(x);
+    uint8_t* dst = static_cast<uint8_t*>(q);
+    if (vectors<T>(x, ldx, 0)) SHARPI_LAUNCH_PDL((fp8_rows_kernel<T, true>), grid, ROWS_WARPS * 32, 0, stream, src, ldx, rows, M, K, dst, ldq, scale);
+    else SHARPI_LAUNCH_PDL((fp8_rows_kernel<T, false>), grid, ROWS_WARPS * 32, 0, stream, src, ldx, rows, M, K, dst, ldq, scale);
+    return SHARPI_OK;
+}
+
+template <typename T>
+int weight_impl(const void* w, int E, int N, int K, long long ldw, long long group, void* q, long long ldq, float* scale, cudaStream_t stream) {
+    const dim3 grid((K + fp8::BLOCK - 1) / fp8::BLOCK, (N + fp8::BLOCK - 1) / fp8::BLOCK, E);
+    if (grid.y > 65535 || grid.z > 65535) return SHARPI_BAD_ARGUMENT;
+    const T* src = static_cast<const T*>(w);
+    uint8_t* dst = static_cast<uint8_t*>(q);
+    if (vectors<T>(w, ldw, group)) SHARPI_LAUNCH_PDL((fp8_weight_kernel<T, true>), grid, WEIGHT_THREADS, 0, stream, src, N, K, ldw, group, dst, ldq, scale);
+    else SHARPI_LAUNCH_PDL((fp8_weight_kernel<T, false>), grid, WEIGHT_THREADS, 0, stream, src, N, K, ldw, group, dst, ldq, scale);
+    return SHARPI_OK;
+}
+
+}  // namespace
+
+SHARPI_API int sharpi_fp8_rows(const void* x, int dtype, long long ldx, const int* rows, int M, int K, void* q, long long ldq,
+                               float* scale, cudaStream_t stream) {
+    if (M <= 0 || K <= 0) return SHARPI_OK;
+    if (ldq < K || ldq % 16 != 0 || (reinterpret_cast<uintptr_t>(q) & 15) || (reinterpret_cast<uintptr_t>(scale) & 15)) return SHARPI_UNALIGNED;
+    return dtype == SHARPI_BF16 ? rows_impl<bf16>(x, ldx, rows, M, K, q, ldq, scale, stream)
+         : dtype == SHARPI_F32 ? rows_impl<float>(x, ldx, rows, M, K, q, ldq, scale, stream) : (int)SHARPI_BAD_ARGUMENT;
+}
+
+SHARPI_API int sharpi_fp8_weight(const void* w, int dtype, int E, int N, int K, long long ldw, long long group, void* q,
+                                 long long ldq, float* scale, cudaStream_t stream) {
+    if (E <= 0 || N <= 0 || K <= 0) return SHARPI_OK;
+    if (ldq < K || ldq % 16 != 0 || (reinterpret_cast<uintptr_t>(q) & 15)) return SHARPI_UNALIGNED;
+    return dtype == SHARPI_BF16 ? weight_impl<bf16>(w, E, N, K, ldw, group, q, ldq, scale, stream)
+         : dtype == SHARPI_F32 ? weight_impl<float>(w, E, N, K, ldw, group, q, ldq, scale, stream) : (int)SHARPI_BAD_ARGUMENT;
+}

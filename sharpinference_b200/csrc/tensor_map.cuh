@@ -54,4 +54,19 @@ inline bool make_bf16_rows_map(CUtensorMap* map, const void* base, uint64_t d0, 
               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// 8-bit tensor [d2][d1][d0] with rows ld bytes apart (a multiple of 16) and d1 * ld between the outermost (d2 == 0 makes it
+// two-dimensional): boxes of [1, box1, 128], 128-byte swizzle, out-of-range elements read as zero.
+inline bool make_u8_map(CUtensorMap* map, const void* base, uint64_t d0, uint64_t d1, uint64_t d2, uint64_t ld, uint32_t box1) {
+    EncodeTiledFn fn = encode_tiled();
+    if (!fn) return false;
+    const bool three = d2 > 0;
+    cuuint64_t dims[3] = {d0, d1, three ? d2 : 1};
+    cuuint64_t strides[2] = {ld, d1 * ld};
+    cuuint32_t box[3] = {128, box1, 1};
+    cuuint32_t elem[3] = {1, 1, 1};
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, three ? 3 : 2, const_cast<void*>(base), dims, strides, box, elem,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 }  // namespace tmap

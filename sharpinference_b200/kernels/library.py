@@ -104,6 +104,9 @@ SIGNATURES: Dict[str, Tuple[str, list]] = {
     "sharpi_delta_walk": ("delta", [P, P, P, I, P, P, P, P, P, I, I, P, LL, P, I, I, I, I, P]),
     "sharpi_delta_chunks": ("delta", [P, P, P, I, P, P, P, P, P, I, P, I, P, P, P, P, LL, P, I, I, I, I, I, P]),
     "sharpi_head_norm_gate": ("delta", [P, P, I, P, F, I, I, I, P, I, P]),
+    "sharpi_fp8_rows": ("fp8_quant", [P, I, LL, P, I, I, P, LL, P, P]),
+    "sharpi_fp8_weight": ("fp8_quant", [P, I, I, I, I, LL, LL, P, LL, P, P]),
+    "sharpi_fp8_gemm": ("fp8_gemm", [P, LL, P, P, LL, P, P, P, P, P, P, P, LL, P, P, I, I, I, I, I, I, I, I, P]),
     "sharpi_gated_group_norm": ("mamba2", [P, P, I, P, F, I, I, I, P, I, P]),
 }
 

@@ -526,8 +526,8 @@ def check_status(device) -> None:
                 buf.zero_()               # a kernel that gave up may have left counters behind
             raise KernelError(f"a tensor-core kernel gave up (code {code}: 1 = wait for a free stage, 2 = for a loaded "
                               f"stage, 3 = for the accumulator, 4 = for a key/value copy, 5 = misaligned staging "
-                              f"buffer, 6 = misaligned shared memory, 7 = for drained tensor memory, 11-18 = "
-                              f"attention: queries, keys, values, scores, probabilities, outputs, free stage, "
+                              f"buffer, 6 = misaligned shared memory, 7 = for drained tensor memory, 8 = for a block's "
+                              f"scales, 11-18 = attention: queries, keys, values, scores, probabilities, outputs, free stage, "
                               f"misaligned shared memory); its output is incomplete")
 
 
@@ -2092,3 +2092,196 @@ def head_norm_gate(y: torch.Tensor, gate: torch.Tensor, weight: torch.Tensor, ep
     check(kernel("sharpi_head_norm_gate")(y.data_ptr(), gate.data_ptr(), ld, weight.data_ptr(), float(eps), T, heads, n // heads,
                                           out.data_ptr(), dtype_code(out_dtype), _stream()), "sharpi_head_norm_gate")
     return out
+
+
+# ---------------------------------------------------------------------------------------
+# block-scaled 8-bit operands: e4m3 values with a float32 scale for 128 neighbours of a row (activations) or for 128 x 128
+# (weights); scale = max(amax / 448, 2^-126), q = e4m3(x / scale).  A NaN or an infinity makes its block NaN.
+# ---------------------------------------------------------------------------------------
+FP8 = torch.float8_e4m3fn
+FP8_BLOCK = 128
+
+
+def fp8_blocks(n: int) -> int:
+    """Blocks of 128 along ``n`` elements."""
+    return (n + FP8_BLOCK - 1) // FP8_BLOCK
+
+
+def _here(*tensors) -> None:
+    """All tensors given (or None) lie on the current device, on whose stream the kernels are launched."""
+    here = torch._C._cuda_getDevice()
+    for t in tensors:
+        if t is not None and t.get_device() != here:
+            raise KernelError(f"a tensor is on {t.device}, the current device is cuda:{here}")
+
+
+def fp8_empty(shape: Sequence[int], device) -> torch.Tensor:
+    """An e4m3 tensor whose rows start on 16-byte boundaries (the bytes between the rows are not set)."""
+    K = shape[-1]
+    if K % 16 == 0:
+        return torch.empty(shape, dtype=FP8, device=device)
+    return torch.empty((*shape[:-1], (K + 15) // 16 * 16), dtype=FP8, device=device)[..., :K]
+
+
+def _need_fp8(q: torch.Tensor, scale: torch.Tensor, name: str, dims: int, scale_shape) -> int:
+    """The bytes between two rows of an 8-bit operand; raises where the products do not take it."""
+    if not q.is_cuda:
+        raise KernelError(f"{name} must be a CUDA tensor (the engine has no CPU path); found device {q.device}")
+    if q.dtype != FP8:
+        raise KernelError(f"{name} must have dtype {FP8}, found {q.dtype}")
+    if q.dim() != dims:
+        raise KernelError(f"{name} must have {dims} dimensions, found shape {tuple(q.shape)}")
+    K = q.shape[-1]
+    ld = q.stride(-2) if q.shape[-2] > 1 else (K + 15) // 16 * 16
+    if (K > 1 and q.stride(-1) != 1) or ld < K or (dims == 3 and q.shape[0] > 1 and q.stride(0) != ld * q.shape[1]):
+        raise KernelError(f"the rows of {name} must be contiguous and equally far apart, found strides {q.stride()} for shape {tuple(q.shape)}")
+    if ld % 16 or q.data_ptr() % 16:
+        raise KernelError(f"the rows of {name} must start on 16-byte boundaries, as fp8_rows, fp8_weight and fp8_empty lay "
+                          f"them; found rows {ld} bytes apart")
+    _need(scale, f"{name}_scale", torch.float32)
+    if tuple(scale.shape) != tuple(scale_shape):
+        raise KernelError(f"{name}_scale is {tuple(scale.shape)}, expected {tuple(scale_shape)}")
+    return ld
+
+
+def fp8_rows(x: torch.Tensor, *, rows: Optional[torch.Tensor] = None):
+    """Activations in 8 bits: ``x`` float32 or bfloat16 ``[T, K]`` (rows contiguous, possibly lying apart) becomes ``(q e4m3
+    [M, K], scale float32 [blocks, M])``, a scale for 128 neighbours of a row.  ``rows`` (int32 ``[M]``) names the rows to
+    take (a mixture's sorted rows); without it all are."""
+    ld = _need_columns(x, "x")
+    dtype = dtype_code(x.dtype)
+    if rows is not None:
+        _need(rows, "rows", torch.int32)
+        if rows.dim() != 1:
+            raise KernelError(f"rows must have one dimension, found shape {tuple(rows.shape)}")
+    _here(x, rows)
+    T, K = x.shape
+    M = T if rows is None else rows.numel()
+    if K == 0 or (M > 0 and T == 0):
+        raise KernelError(f"x is {tuple(x.shape)}: no elements to quantise")
+    q = fp8_empty((M, K), x.device)
+    scale = torch.empty((fp8_blocks(K), M), dtype=torch.float32, device=x.device)
+    check(kernel("sharpi_fp8_rows")(x.data_ptr(), dtype, ld, _ptr(rows), M, K, q.data_ptr(), (K + 15) // 16 * 16, scale.data_ptr(),
+                                    _stream()), "sharpi_fp8_rows")
+    return q, scale
+
+
+def fp8_weight(w: torch.Tensor):
+    """A weight in 8 bits: ``w`` float32 or bfloat16 ``[N, K]`` or ``[E, N, K]`` becomes ``(q e4m3 of that shape, scale float32
+    [(E,) blocks of N, blocks of K])``, a scale for 128 x 128."""
+    if not w.is_cuda:
+        raise KernelError(f"w must be a CUDA tensor (the engine has no CPU path); found device {w.device}")
+    if w.dim() not in (2, 3) or (w.shape[-1] > 1 and w.stride(-1) != 1):
+        raise KernelError(f"w must be [N, K] or [E, N, K] with contiguous rows, found shape {tuple(w.shape)}, strides {w.stride()}")
+    dtype = dtype_code(w.dtype)
+    _here(w)
+    N, K = w.shape[-2:]
+    E = w.shape[0] if w.dim() == 3 else 1
+    if K == 0:
+        raise KernelError(f"w is {tuple(w.shape)}: no elements to quantise")
+    q = fp8_empty(w.shape, w.device)
+    scale = torch.empty((*w.shape[:-2], fp8_blocks(N), fp8_blocks(K)), dtype=torch.float32, device=w.device)
+    check(kernel("sharpi_fp8_weight")(w.data_ptr(), dtype, E, N, K, w.stride(-2) if N > 1 else K, w.stride(0) if E > 1 else 0,
+                                      q.data_ptr(), (K + 15) // 16 * 16, scale.data_ptr(), _stream()), "sharpi_fp8_weight")
+    return q, scale
+
+
+_OUT_DTYPES = (torch.float32, torch.bfloat16)
+
+
+def _fp8_product(a, a_scale, w, w_scale, group_offsets, *, swiglu=False, out=None, out_scale=None, out_dtype=torch.float32,
+                 out_rows=None, row_scale=None, scale_rows=None, bias=None, accumulate=False):
+    if a.dim() != 2 or w.dim() not in (2, 3) or a.shape[1] != w.shape[-1] or a.shape[1] == 0:
+        raise KernelError(f"inner sizes differ or shapes are not [rows, K] and [N, K] or [E, N, K]: a {tuple(a.shape)}, w {tuple(w.shape)}")
+    rows, K = a.shape
+    N, E = w.shape[-2], (w.shape[0] if w.dim() == 3 else 1)
+    lda = _need_fp8(a, a_scale, "a", 2, (fp8_blocks(K), rows))
+    ldw = _need_fp8(w, w_scale, "w", w.dim(), (*w.shape[:-2], fp8_blocks(N), fp8_blocks(K)))
+    if (group_offsets is None) != (w.dim() == 2):
+        raise KernelError("group_offsets [E + 1] belong to weights [E, N, K], and weights [N, K] have none")
+    if group_offsets is not None:
+        _need(group_offsets, "group_offsets", torch.int32)
+        if group_offsets.numel() != E + 1:
+            raise KernelError(f"group_offsets has {group_offsets.numel()} entries for {E} experts")
+    if out_rows is not None:
+        _need(out_rows, "out_rows", torch.int32)
+        if out_rows.numel() < rows:
+            raise KernelError(f"out_rows has {out_rows.numel()} entries for {rows} rows")
+    if scale_rows is not None:
+        _need(scale_rows, "scale_rows", torch.int32)
+        if scale_rows.numel() < rows:
+            raise KernelError(f"scale_rows has {scale_rows.numel()} entries for {rows} rows")
+    if row_scale is not None:
+        _need(row_scale, "row_scale", torch.float32)
+        if scale_rows is None and row_scale.numel() < rows:
+            raise KernelError(f"row_scale has {row_scale.numel()} entries for {rows} rows")
+    if scale_rows is not None and row_scale is None:
+        raise KernelError("scale_rows say which row_scale a row has: there is none")
+    if bias is not None:
+        _need(bias, "bias", torch.float32)
+        if bias.numel() != N:
+            raise KernelError(f"bias has {bias.numel()} entries, the product has {N} columns")
+    if out is None:
+        if accumulate:
+            raise KernelError("accumulate=True needs an output tensor to add to")
+        if out_dtype not in _OUT_DTYPES:
+            raise KernelError(f"out_dtype {out_dtype} is not one of {_OUT_DTYPES}")
+        out = torch.empty((rows, N), dtype=out_dtype, device=a.device)
+    elif not swiglu:
+        _need(out, "out")
+        if out.dtype not in _OUT_DTYPES or (accumulate and out.dtype != torch.float32):
+            raise KernelError(f"out must be float32{'' if accumulate else ' or bfloat16'}, found {out.dtype}")
+        if out.dim() != 2 or out.shape[1] != N or (out_rows is None and out.shape[0] < rows):
+            raise KernelError(f"out is {tuple(out.shape)} for a product of {rows} rows and {N} columns")
+    _here(a, a_scale, w, w_scale, group_offsets, out, out_rows, row_scale, scale_rows, bias)
+    if rows == 0 or N == 0 or E == 0:
+        return out
+    check(kernel("sharpi_fp8_gemm")(a.data_ptr(), lda, a_scale.data_ptr(), w.data_ptr(), ldw, w_scale.data_ptr(), _ptr(group_offsets),
+                                    _ptr(out_rows), _ptr(row_scale), _ptr(scale_rows), _ptr(bias), out.data_ptr(),
+                                    out.stride(0) if swiglu else 0, _ptr(out_scale), status_word(a.device).data_ptr(), rows, N, K, E,
+                                    int(swiglu), int(out.dtype == torch.bfloat16), int(accumulate), sm_count(a.device), _stream()),
+          "sharpi_fp8_gemm")
+    return out
+
+
+def fp8_dense(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, *, bias: Optional[torch.Tensor] = None,
+              out: Optional[torch.Tensor] = None, out_dtype: torch.dtype = torch.float32, accumulate: bool = False) -> torch.Tensor:
+    """``a . w^T (+ bias)`` of block-scaled 8-bit operands: ``a`` e4m3 ``[M, K]`` with ``a_scale [blocks of K, M]`` (from
+    :func:`fp8_rows`), ``w`` e4m3 ``[N, K]`` with ``w_scale [blocks of N, blocks of K]`` (from :func:`fp8_weight`).  Sums are
+    float32; ``[M, N]`` float32 or bfloat16, or added into float32 ``out`` when ``accumulate``."""
+    if w.dim() != 2:
+        raise KernelError(f"a dense product needs w [N, K], found {tuple(w.shape)}")
+    return _fp8_product(a, a_scale, w, w_scale, None, bias=bias, out=out, out_dtype=out_dtype, accumulate=accumulate)
+
+
+def fp8_grouped(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, group_offsets: torch.Tensor, *,
+                out: Optional[torch.Tensor] = None, out_dtype: torch.dtype = torch.float32, out_rows: Optional[torch.Tensor] = None,
+                row_scale: Optional[torch.Tensor] = None, scale_rows: Optional[torch.Tensor] = None,
+                accumulate: bool = False) -> torch.Tensor:
+    """Per-expert products of block-scaled 8-bit operands: ``a`` e4m3 ``[rows, K]`` sorted by expert, ``w`` e4m3 ``[E, N, K]``,
+    ``group_offsets`` int32 ``[E + 1]``; scales as in :func:`fp8_dense`.  ``out[out_rows[r] or r] (+)= s * a[r] . w[e(r)]^T`` with
+    ``s = row_scale[scale_rows[r] or r]`` or 1, as in :func:`tc_grouped_gemm`.  Rows behind ``group_offsets[E]`` belong to no
+    expert and are not written.  Two rows must not share an entry of ``out_rows``."""
+    if w.dim() != 3:
+        raise KernelError(f"a grouped product needs w [E, N, K], found {tuple(w.shape)}")
+    return _fp8_product(a, a_scale, w, w_scale, group_offsets, out=out, out_dtype=out_dtype, out_rows=out_rows, row_scale=row_scale,
+                        scale_rows=scale_rows, accumulate=accumulate)
+
+
+def fp8_swiglu(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor,
+               group_offsets: Optional[torch.Tensor] = None, *, row_scale: Optional[torch.Tensor] = None,
+               scale_rows: Optional[torch.Tensor] = None):
+    """The first product of gated networks with SwiGLU and the quantisation for the second one in its epilogue: ``w`` holds gate
+    rows then up rows (``[2 I, K]``, or ``[E, 2 I, K]`` with ``group_offsets`` for experts), ``h = silu(s g) * (s u)`` with ``s =
+    row_scale[scale_rows[r] or r]`` or 1; returns ``(q e4m3 [rows, I], scale [blocks of I, rows])``, what :func:`fp8_rows` would
+    make of ``h``.  Where ``I`` is no multiple of 128 the product, SwiGLU and the quantisation are a kernel each."""
+    if w.dim() not in (2, 3) or w.shape[-2] % 2:
+        raise KernelError(f"a SwiGLU product needs w [2 I, K] or [E, 2 I, K], found {tuple(w.shape)}")
+    rows, I = a.shape[0], w.shape[-2] // 2
+    if I % FP8_BLOCK or I == 0:
+        gate_up = _fp8_product(a, a_scale, w, w_scale, group_offsets, row_scale=row_scale, scale_rows=scale_rows)
+        return fp8_rows(swiglu(gate_up, torch.float32))
+    q = fp8_empty((rows, I), a.device)
+    scale = torch.empty((I // FP8_BLOCK, rows), dtype=torch.float32, device=a.device)
+    _fp8_product(a, a_scale, w, w_scale, group_offsets, swiglu=True, out=q, out_scale=scale, row_scale=row_scale, scale_rows=scale_rows)
+    return q, scale
