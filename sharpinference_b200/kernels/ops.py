@@ -528,7 +528,7 @@ def check_status(device) -> None:
                               f"stage, 3 = for the accumulator, 4 = for a key/value copy, 5 = misaligned staging "
                               f"buffer, 6 = misaligned shared memory, 7 = for drained tensor memory, 8 = for a block's "
                               f"scales, 11-18 = attention: queries, keys, values, scores, probabilities, outputs, free stage, "
-                              f"misaligned shared memory); its output is incomplete")
+                              f"misaligned shared memory, 19 = for the other blocks of a mixture layer); its output is incomplete")
 
 
 TC_MODE_STORE, TC_MODE_SWIGLU = 0, 1
@@ -2285,3 +2285,104 @@ def fp8_swiglu(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale:
     scale = torch.empty((I // FP8_BLOCK, rows), dtype=torch.float32, device=a.device)
     _fp8_product(a, a_scale, w, w_scale, group_offsets, swiglu=True, out=q, out_scale=scale, row_scale=row_scale, scale_rows=scale_rows)
     return q, scale
+
+
+MOE_FEW_TOKENS = 16
+
+
+def _need_rows_16(w: torch.Tensor, name: str) -> int:
+    """Bytes between the rows of a weight ``[E, N, K]``, which start on 16-byte boundaries."""
+    size = w.element_size()
+    ld = (w.stride(1) if w.shape[1] > 1 else (w.shape[2] * size + 15) // 16 * 16 // size) * size
+    if (w.shape[2] > 1 and w.stride(2) != 1) or ld < w.shape[2] * size or (w.shape[0] > 1 and w.stride(0) * size != ld * w.shape[1]):
+        raise KernelError(f"the rows of {name} must be contiguous and equally far apart, found strides {w.stride()} for shape {tuple(w.shape)}")
+    if ld % 16 or w.data_ptr() % 16:
+        raise KernelError(f"the rows of {name} must start on 16-byte boundaries, found rows {ld} bytes apart")
+    return ld
+
+
+def moe_few(h: torch.Tensor, router_weight: torch.Tensor, gate_up: torch.Tensor, down: torch.Tensor, k: int, *,
+            h32: Optional[torch.Tensor] = None, gate_up_scale: Optional[torch.Tensor] = None, down_scale: Optional[torch.Tensor] = None,
+            correction: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None, scoring: str = "sigmoid",
+            renormalize: bool = False, scale: float = 1.0, weights_on: str = "output", add: Optional[torch.Tensor] = None,
+            out: Optional[torch.Tensor] = None, out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """A whole mixture layer for up to 16 tokens in two kernels: router, choice of ``k`` gated experts a token, both products and
+    the weighted sum; ``[T, H]`` float32 or bfloat16.
+
+    ``h`` bfloat16 ``[T, H]``; ``h32`` (float32, optional) are the unrounded activations, which the router reads instead.
+    Choice and weights (``router_weight``, ``correction``, ``bias``, ``scoring``, ``renormalize``, ``scale``) as in
+    :func:`router_topk`; a NaN among a token's logits makes its output NaN.  ``gate_up`` ``[E, 2 I, H]`` holds gate rows then up
+    rows, ``down`` is ``[E, H, I]``: both bfloat16 with ``H`` and ``I`` multiples of 8, or both e4m3 with the scales of
+    :func:`fp8_weight` and an even ``I``.  ``weights_on``: a weight multiplies its expert's ``"input"`` (before the nonlinearity) or
+    ``"output"``.  ``add`` float32 ``[T, H]`` is added (a shared expert's output; ``out`` may be it).
+
+    ``silu(g) * u`` is rounded to bfloat16 between the products, everything else is float32.  The order in which a token's terms
+    are added goes by the experts that the whole call reaches."""
+    _need(h, "h", torch.bfloat16)
+    _need(router_weight, "router_weight", torch.float32)
+    if h.dim() != 2 or router_weight.dim() != 2 or gate_up.dim() != 3 or down.dim() != 3:
+        raise KernelError(f"expected h [T, H], router [E, H], gate_up [E, 2 I, H] and down [E, H, I], found {tuple(h.shape)}, "
+                          f"{tuple(router_weight.shape)}, {tuple(gate_up.shape)}, {tuple(down.shape)}")
+    (T, H), (E, I) = h.shape, (down.shape[0], down.shape[2])
+    if tuple(router_weight.shape) != (E, H) or tuple(gate_up.shape) != (E, 2 * I, H) or tuple(down.shape) != (E, H, I) or not H * I:
+        raise KernelError(f"shapes disagree: h {tuple(h.shape)}, router {tuple(router_weight.shape)}, gate_up {tuple(gate_up.shape)}, "
+                          f"down {tuple(down.shape)}")
+    if T > MOE_FEW_TOKENS:
+        raise KernelError(f"moe_few takes up to {MOE_FEW_TOKENS} tokens, found {T}")
+    if not (1 <= k <= min(E, 32)) or E > 1024:
+        raise KernelError(f"experts per row must be 1 .. min(experts, 32) of up to 1024, found {k} of {E}")
+    w8 = gate_up_scale is not None
+    if w8 != (down_scale is not None):
+        raise KernelError("gate_up and down both have scales or neither has")
+    if w8:
+        ldg = _need_fp8(gate_up, gate_up_scale, "gate_up", 3, (E, fp8_blocks(2 * I), fp8_blocks(H)))
+        ldd = _need_fp8(down, down_scale, "down", 3, (E, fp8_blocks(H), fp8_blocks(I)))
+        if I % 2:
+            raise KernelError(f"the experts' width must be even, found {I}")
+    else:
+        for name, w in (("gate_up", gate_up), ("down", down)):
+            if not w.is_cuda or w.dtype != torch.bfloat16:
+                raise KernelError(f"{name} must be a bfloat16 CUDA tensor, or e4m3 with its scales; found {w.dtype} on {w.device}")
+        if H % 8 or I % 8:
+            raise KernelError(f"bfloat16 experts need widths that are multiples of 8, found {H} and {I}")
+        ldg, ldd = _need_rows_16(gate_up, "gate_up"), _need_rows_16(down, "down")
+    if scoring not in ROUTER_SCORING:
+        raise KernelError(f"router scoring '{scoring}' is not one of {', '.join(ROUTER_SCORING)}")
+    if weights_on not in ("input", "output"):
+        raise KernelError(f"weights_on '{weights_on}' is not one of input, output")
+    for name, t in (("correction", correction), ("bias", bias)):
+        if t is not None:
+            _need(t, name, torch.float32)
+            if t.numel() != E:
+                raise KernelError(f"{name} has {t.numel()} entries for {E} experts")
+    for name, t in (("h32", h32), ("add", add)):
+        if t is not None:
+            _need(t, name, torch.float32)
+            if tuple(t.shape) != (T, H):
+                raise KernelError(f"{name} is {tuple(t.shape)}, expected {(T, H)}")
+    if out is None:
+        if out_dtype not in _OUT_DTYPES:
+            raise KernelError(f"out_dtype {out_dtype} is not one of {_OUT_DTYPES}")
+        out = torch.empty((T, H), dtype=out_dtype, device=h.device)
+    else:
+        _need(out, "out")
+        if out.dtype not in _OUT_DTYPES or tuple(out.shape) != (T, H):
+            raise KernelError(f"out is {out.dtype} {tuple(out.shape)}, expected float32 or bfloat16 {(T, H)}")
+    _here(h, router_weight, gate_up, down, h32, gate_up_scale, down_scale, correction, bias, add, out)
+    if T == 0:
+        return out
+    if H % 16 and w8:                     # rows of whole 16-element pieces, zeros behind the end
+        rows = torch.nn.functional.pad(h, (0, -H % 16))
+    else:
+        rows = h
+    x = rows if h32 is None else h32
+    act = min(E, T * k) * T * ((I + 15) // 16 * 16) * 2
+    work = torch.empty(act + 4 * T * E + 4, dtype=torch.uint8, device=h.device)       # act, logits, the barrier's counter
+    at = work.data_ptr()
+    check(kernel("sharpi_moe_few")(x.data_ptr(), dtype_code(x.dtype), x.shape[1], rows.data_ptr(), rows.shape[1], router_weight.data_ptr(),
+                                   _ptr(bias), _ptr(correction), gate_up.data_ptr(), ldg, _ptr(gate_up_scale), down.data_ptr(), ldd,
+                                   _ptr(down_scale), _ptr(add), at + act, at, at + act + 4 * T * E, status_word(h.device).data_ptr(),
+                                   out.data_ptr(), int(out.dtype == torch.bfloat16), T, E, k, H, I, ROUTER_SCORING[scoring],
+                                   int(renormalize), float(scale), int(weights_on == "input"), sm_count(h.device), _stream()),
+          "sharpi_moe_few")
+    return out

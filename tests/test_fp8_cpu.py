@@ -1,4 +1,4 @@
-"""What the block-scaled 8-bit operators refuse, without a GPU: tensors that say they are on the device, and kernels that
+"""What the block-scaled 8-bit operators and the mixture layer for a few tokens refuse, without a GPU: tensors that say they are on the device, and kernels that
 only note that they were called."""
 import pytest
 import torch
@@ -121,10 +121,69 @@ def test_refused(calls, name):
     assert not calls
 
 
+def few(T=3, E=6, H=64, I=32, k=2, w8=False, **more):
+    """A call of moe_few with some of its arguments replaced."""
+    args = {"h": dev(torch.zeros(T, H, dtype=BF16)), "router": dev(torch.zeros(E, H)),
+            "gate_up": dev(ops.fp8_empty((E, 2 * I, H), "cpu") if w8 else torch.zeros(E, 2 * I, H, dtype=BF16)),
+            "down": dev(ops.fp8_empty((E, H, I), "cpu") if w8 else torch.zeros(E, H, I, dtype=BF16))}
+    if w8:
+        args["gate_up_scale"] = dev(torch.ones(E, ops.fp8_blocks(2 * I), ops.fp8_blocks(H)))
+        args["down_scale"] = dev(torch.ones(E, ops.fp8_blocks(H), ops.fp8_blocks(I)))
+    args.update(more)
+    return ops.moe_few(args.pop("h"), args.pop("router"), args.pop("gate_up"), args.pop("down"), k, **args)
+
+
+def test_few_calls_that_are_taken(calls):
+    few()
+    few(w8=True, H=63, I=34)
+    few(T=16, k=6, bias=dev(torch.zeros(6)), correction=dev(torch.zeros(6)), scoring="softmax_chosen", weights_on="input", out_dtype=BF16)
+    assert [s for s, _ in calls] == ["sharpi_moe_few"] * 3
+
+
+FEW_REFUSED = {
+    "on_the_cpu": dict(h=torch.zeros(3, 64, dtype=BF16)),
+    "float32_rows": dict(h=dev(torch.zeros(3, 64))),
+    "17_tokens": dict(T=17),
+    "no_experts_a_token": dict(k=0),
+    "more_experts_a_token_than_there_are": dict(k=7),
+    "33_experts_a_token": dict(E=40, k=33),
+    "1025_experts": dict(E=1025, H=8, I=8),
+    "router_shape": dict(router=dev(torch.zeros(5, 64))),
+    "router_bf16": dict(router=dev(torch.zeros(6, 64, dtype=BF16))),
+    "gate_up_shape": dict(gate_up=dev(torch.zeros(6, 63, 64, dtype=BF16))),
+    "gate_up_float32": dict(gate_up=dev(torch.zeros(6, 64, 64))),
+    "down_shape": dict(down=dev(torch.zeros(6, 32, 64, dtype=BF16))),
+    "down_on_the_cpu": dict(down=torch.zeros(6, 64, 32, dtype=BF16)),
+    "widths_of_bf16_weights": dict(H=60),
+    "inner_width_of_bf16_weights": dict(I=28),
+    "odd_inner_width": dict(w8=True, I=33),
+    "one_scale_alone": dict(w8=True, down_scale=None),
+    "scale_shape": dict(w8=True, down_scale=dev(torch.ones(6, 2, 1))),
+    "8_bit_weights_without_scales": dict(w8=True, gate_up_scale=None, down_scale=None),
+    "rows_off_16_bytes": dict(gate_up=dev(torch.zeros(6, 64, 68, dtype=BF16)[..., 4:])),
+    "rows_apart_unevenly": dict(gate_up=dev(torch.zeros(6, 70, 64, dtype=BF16)[:, :64])),
+    "unknown_scoring": dict(scoring="softmax"),
+    "unknown_place_of_weights": dict(weights_on="both"),
+    "bias_size": dict(bias=dev(torch.zeros(5))),
+    "correction_dtype": dict(correction=dev(torch.zeros(6, dtype=BF16))),
+    "h32_shape": dict(h32=dev(torch.zeros(2, 64))),
+    "add_bf16": dict(add=dev(torch.zeros(3, 64, dtype=BF16))),
+    "out_shape": dict(out=dev(torch.zeros(3, 65))),
+    "out_float16": dict(out_dtype=torch.float16),
+}
+
+
+@pytest.mark.parametrize("name", sorted(FEW_REFUSED))
+def test_few_refused(calls, name):
+    with pytest.raises(KernelError):
+        few(**FEW_REFUSED[name])
+    assert not calls
+
+
 def test_another_device_is_refused(calls, monkeypatch):
     monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 1)
     for call in (lambda: ops.fp8_rows(dev(torch.zeros(5, 200))), lambda: ops.fp8_weight(dev(torch.zeros(5, 200))),
-                 lambda: ops.fp8_dense(*operands()), lambda: ops.fp8_swiglu(*operands(N=256))):
+                 lambda: ops.fp8_dense(*operands()), lambda: ops.fp8_swiglu(*operands(N=256)), few):
         with pytest.raises(KernelError, match="current device"):
             call()
     assert not calls

@@ -1,0 +1,200 @@
+"""The mixture layer for a few tokens against a plain statement in 64 bits (needs a GPU)."""
+import pytest
+import torch
+
+from plain_fp8 import F64, weight_of
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda:0"
+BF16, F32 = torch.bfloat16, torch.float32
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from sharpinference_b200.kernels import ops as _ops
+    yield _ops
+    _ops.check_status(DEV)
+
+
+def rnd(*shape, dtype=F32, scale=1.0, seed=0):
+    g = torch.Generator(device="cpu").manual_seed(seed)
+    return (torch.randn(*shape, generator=g) * scale).to(dtype).to(DEV)
+
+
+def layer(ops, T, E, H, I, weights="bfloat16", seed=0):
+    h32 = rnd(T, H, scale=1.5, seed=seed)
+    c = {"h": h32.to(BF16), "h32": h32, "router": rnd(E, H, scale=H ** -0.5, seed=seed + 1)}
+    gate_up, down = rnd(E, 2 * I, H, scale=H ** -0.5, seed=seed + 2), rnd(E, H, I, scale=I ** -0.5, seed=seed + 3)
+    if weights == "e4m3":
+        c["gate_up"], c["gate_up_scale"] = ops.fp8_weight(gate_up)
+        c["down"], c["down_scale"] = ops.fp8_weight(down)
+    else:
+        c["gate_up"], c["down"], c["gate_up_scale"], c["down_scale"] = gate_up.to(BF16), down.to(BF16), None, None
+    return c
+
+
+def call(ops, c, k, **more):
+    return ops.moe_few(c["h"], c["router"], c["gate_up"], c["down"], k, h32=c["h32"], gate_up_scale=c["gate_up_scale"],
+                       down_scale=c["down_scale"], **more)
+
+
+def plain(c, expert, weight, on):
+    """``(y, bound)``: the layer in 64 bits under the given choices, and a bound on the kernel's error: float32 sums of n
+    terms (n 2^-24 of the sum of magnitudes at most), silu's slope at most 1.1, one rounding of act to bfloat16 (2^-8)."""
+    h = c["h"].to(F64)
+    T, H = h.shape
+    y, bound = torch.zeros_like(h), torch.zeros_like(h)
+    W = {n: c[n].to(F64) if c[n + "_scale"] is None else weight_of(c[n], c[n + "_scale"]) for n in ("gate_up", "down")}
+    I = W["down"].shape[2]
+    for t in range(T):
+        for e, w in zip(expert[t].tolist(), weight[t].to(F64).tolist()):
+            gu = W["gate_up"][e] @ h[t]
+            err = (H + 8) * 2.0 ** -24 * (W["gate_up"][e].abs() @ h[t].abs())
+            if on == "input":
+                gu, err = gu * w, err * abs(w) + gu.abs() * abs(w) * 2.0 ** -24
+            g, u = gu[:I], gu[I:]
+            act = g * torch.sigmoid(g) * u
+            err = 1.1 * err[:I] * u.abs() + g.abs() * err[I:] + act.abs() * (8 + g.abs()) * 2.0 ** -23
+            if on == "output":
+                act, err = act * w, err * abs(w) + act.abs() * abs(w) * 2.0 ** -24
+            err = err + act.abs() * 2.0 ** -8
+            y[t] += W["down"][e] @ act
+            bound[t] += W["down"][e].abs() @ (err + (I * expert.shape[1] + 40) * 2.0 ** -24 * act.abs())
+    return y, bound
+
+
+def close(got, want, bound):
+    if got.dtype == BF16:
+        bound = bound + (want.abs() + bound) * 2.0 ** -8
+    bad = ~((got.to(F64) - want).abs() <= bound)
+    assert not bad.any(), f"{int(bad.sum())} of {bad.numel()} beyond, worst {float(((got.to(F64) - want).abs() / bound.clamp_min(1e-300)).max()):.3g} of the bound"
+
+
+@pytest.mark.parametrize("weights", ["bfloat16", "e4m3"])
+@pytest.mark.parametrize("T,E,k,H,I", [(1, 8, 2, 128, 64), (1, 128, 8, 2048, 768), (2, 3, 3, 1000, 40), (5, 16, 1, 520, 200), (8, 16, 4, 1024, 512),
+                                       (9, 16, 2, 1024, 136), (16, 64, 8, 640, 384), (16, 4, 4, 256, 1000), (16, 300, 32, 128, 64),
+                                       (3, 1, 1, 64, 8)])
+def test_layer(ops, weights, T, E, k, H, I):
+    c = layer(ops, T, E, H, I, weights, seed=T + E + H)
+    for i, on in enumerate(("input", "output")):
+        for scoring, renormalize in (("sigmoid", bool(i)), ("softmax_chosen", False)):
+            expert, weight, _ = ops.router_topk(c["h32"], c["router"], k, scoring=scoring, renormalize=renormalize, scale=1.3)
+            y, bound = plain(c, expert, weight, on)
+            got = call(ops, c, k, scoring=scoring, renormalize=renormalize, scale=1.3, weights_on=on)
+            assert got.dtype == F32 and tuple(got.shape) == (T, H)
+            close(got, y, bound)
+    close(call(ops, c, k, scoring="softmax_chosen", scale=1.3, out_dtype=BF16), y, bound)
+
+
+@pytest.mark.parametrize("T,H,I", [(1, 257, 130), (11, 1001, 74), (4, 17, 2)])
+def test_odd_widths_of_8_bit_weights(ops, T, H, I):
+    c = layer(ops, T, 6, H, I, "e4m3", seed=H)
+    expert, weight, _ = ops.router_topk(c["h32"], c["router"], 3)
+    close(call(ops, c, 3), *plain(c, expert, weight, "output"))
+
+
+def test_bias_correction_and_router_without_float32(ops):
+    T, E, H, I, k = 7, 12, 256, 128, 3
+    c = layer(ops, T, E, H, I, seed=4)
+    bias, correction = rnd(E, seed=5), rnd(E, seed=6)
+    c["h32"] = None
+    expert, weight, _ = ops.router_topk(c["h"].float(), c["router"], k, bias=bias, correction=correction, renormalize=True)
+    close(call(ops, c, k, bias=bias, correction=correction, renormalize=True), *plain(c, expert, weight, "output"))
+
+
+def test_ties_go_to_the_lowest_index(ops):
+    T, E, H, I = 3, 40, 128, 64
+    c = layer(ops, T, E, H, I, seed=1)
+    c["router"].zero_()
+    expert = torch.arange(4, device=DEV).repeat(T, 1)
+    close(call(ops, c, 4), *plain(c, expert, torch.full((T, 4), 0.5, device=DEV), "output"))
+
+
+def test_add_and_out(ops):
+    T, E, H, I, k = 4, 8, 256, 128, 2
+    c = layer(ops, T, E, H, I, seed=2)
+    y = call(ops, c, k)
+    base = rnd(T, H, seed=3)
+    assert torch.equal(call(ops, c, k, add=base), y + base)
+    buf = base.clone()
+    assert call(ops, c, k, add=buf, out=buf) is buf
+    assert torch.equal(buf, y + base)
+    assert tuple(ops.moe_few(c["h"][:0], c["router"], c["gate_up"], c["down"], k).shape) == (0, H)
+
+
+@pytest.mark.parametrize("weights", ["bfloat16", "e4m3"])
+def test_broken_numbers_stay_with_their_token(ops, weights):
+    T, E, H, I, k = 6, 8, 256, 128, 2
+    c = layer(ops, T, E, H, I, weights, seed=9)
+    whole = call(ops, c, k)
+    for value in (float("nan"), float("inf")):
+        d = dict(c, h=c["h"].clone(), h32=c["h32"].clone())
+        d["h"][2, 7] = d["h32"][2, 7] = value
+        y = call(ops, d, k)
+        assert torch.isnan(y[2]).all()
+        others = [0, 1, 3, 4, 5]
+        assert torch.isfinite(y[others]).all()
+        expert, weight, _ = ops.router_topk(c["h32"], c["router"], k)
+        want, bound = plain(c, expert, weight, "output")
+        close(y[others], want[others], bound[others])
+    assert torch.equal(call(ops, c, k), whole)
+
+
+def test_weights_whose_rows_lie_apart(ops):
+    T, E, H, I, k = 5, 6, 256, 128, 2
+    c = layer(ops, T, E, H, I, seed=12)
+    want = call(ops, c, k)
+    wide = torch.full((E, 2 * I, H + 24), float("nan"), dtype=BF16, device=DEV)
+    wide[..., :H] = c["gate_up"]
+    assert torch.equal(call(ops, dict(c, gate_up=wide[..., :H]), k), want)
+
+
+@pytest.mark.parametrize("weights", ["bfloat16", "e4m3"])
+def test_the_same_again_in_graphs_and_on_streams(ops, weights):
+    T, E, H, I, k = 6, 32, 512, 256, 4
+    c = layer(ops, T, E, H, I, weights, seed=21)
+    want = call(ops, c, k)
+    for _ in range(20):
+        assert torch.equal(call(ops, c, k), want)
+    graphs, outs = [], []
+    for _ in range(2):                                  # two graphs of the same layer, replayed side by side
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(call(ops, c, k))
+        graphs.append(g)
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+        with torch.cuda.stream(streams[2]):
+            side = call(ops, c, k)
+    torch.cuda.synchronize()
+    assert torch.equal(side, want) and all(torch.equal(o, want) for o in outs)
+
+
+def test_beside_the_chain_of_kernels(ops):
+    """The same layer as the parts run it: one launch after the other over sorted rows, in bfloat16."""
+    T, E, H, I, k = 8, 16, 512, 256, 2
+    c = layer(ops, T, E, H, I, seed=30)
+    expert, weight, _ = ops.router_topk(c["h32"], c["router"], k)
+    offsets, pairs = ops.moe_sort(expert.view(-1), E)
+    rows = ops.gather_rows_bf16(c["h"], ops.moe_pair_tokens(pairs, k))
+    ones = torch.ones(T * k, device=DEV)
+    act = ops.tc_grouped_gemm(rows, c["gate_up"], offsets, mode=ops.TC_MODE_SWIGLU, row_scale=ones)
+    y = torch.empty(T * k, H, device=DEV)
+    ops.tc_grouped_gemm(act, c["down"], offsets, mode=ops.TC_MODE_STORE, out=y, out_rows=pairs, row_scale=weight.view(-1), scale_rows=pairs)
+    chain = ops.moe_combine(y, k)
+    want, bound = plain(c, expert, weight, "output")
+    close(call(ops, c, k), want, bound)
+    close(chain, want, bound)
+
+
+def test_a_barrier_that_is_not_reached_is_reported(ops):
+    """Codes of waits that gave up reach the host through the status word."""
+    ops.status_word(DEV).fill_(19)
+    with pytest.raises(ops.KernelError, match="19"):
+        ops.check_status(DEV)
+    ops.check_status(DEV)
