@@ -7,14 +7,18 @@
 // changes with every block the sum leaves tensor memory then and is multiplied and added in float32 registers (fma, one
 // rounding a block).
 //
-// Layout.  A tile is 128 activation rows (the lanes of tensor memory) by TILES * 128 weight rows.  A stage holds 128 bytes
-// of K (one swizzle row) of both operands.  Blocks go to two tensor-memory buffers in turn, so the tensor core works on
-// one block while the block before it is read out.  Sixteen warps read: four groups of four (128 lanes), each with a
-// quarter of the columns, 32 TILES sums a thread in registers; one warp issues the copies, one the MMAs, two multiply the
-// scales of rows and weights into a ring in shared memory (a factor a row and weight tile), so the readers' loop is a load
-// from tensor memory and paired multiply-adds.  The registers go where the sums are (setmaxnreg: 4 x 112 + 32).
-// The grid is one CTA an SM (as many as there are tiles); a CTA walks tiles of all experts, those of one weight tile one
-// after the other, and copies and MMAs of its next tile run while the last one's sums are written.
+// Layout.  A tile is 128 activation rows (the M side of the instruction, the lanes of tensor memory) by two weight tiles of
+// 128 rows.  A stage holds 128 bytes of K (one swizzle row) of both operands.  Blocks go to two tensor-memory buffers in
+// turn, so the tensor core works on one block while the block before it is read out.  Eight warps read: two groups of four
+// (128 lanes), each with half of the columns, a row and 128 sums a thread; one warp issues the copies, one the MMAs, two
+// multiply the scales of rows and weights into a ring in shared memory (a factor a row and weight tile), so the readers' loop
+// is loads from tensor memory and paired multiply-adds with one factor.  The registers go where the sums are (setmaxnreg: 2 x
+// 224 + 56).  4096 x 16384 x 5120: 338 us; sixteen readers with 64 sums each (104 registers, which spill) 356; with the operands
+// swapped (weight rows on the lanes, a factor a column) 650 to 920.
+//
+// Two grids.  Many tiles: one CTA an SM that walks tiles of all experts, those of one weight tile one after the other; copies
+// and MMAs of its next tile run while the last one's sums are written.  Few tiles: a cluster of S CTAs a tile, each with its
+// part of K; the parts meet in the CTAs' shared memory and are added in the order of K, row r by CTA r mod S.
 //
 // Two epilogues:
 //   MODE_STORE   C[out_row, n] = (or +=) s D + bias   float32 or bfloat16; out_row = out_rows[sorted row] or the sorted row,
@@ -33,11 +37,16 @@ namespace {
 
 constexpr int BM = 128;              // activation rows of a tile (the M of the instruction)
 constexpr int WN = 128;              // weight rows of a weight tile: one row of scale blocks
+constexpr int BN = 2 * WN;           // weight rows of a tile (the N of the instruction)
 constexpr int BK = fp8::BLOCK;       // K bytes of a stage
-constexpr int A_BOX = 32;            // rows of an activation copy: a tile with few rows asks for what it has
-constexpr int READERS = 16;          // warps that read tensor memory
+constexpr int READERS = 8;           // warps that read tensor memory
 constexpr int THREADS = 32 * (READERS + 4);
-constexpr int RING = 8;              // blocks of scale factors
+constexpr int A_BYTES = BM * BK, W_BYTES = WN * BK, STAGE = A_BYTES + 2 * W_BYTES, STAGES = 4;
+constexpr int RING = 8;              // blocks of scale factors, [2][BM] floats each
+constexpr int STAGING = READERS * 1024;
+constexpr int BARRIERS = 2 * STAGES + 4 + 2 * RING + 1;
+constexpr int SMEM = STAGES * STAGE + RING * 2 * BM * 4 + STAGING + BARRIERS * 8 + 16 + 1024;
+constexpr int MAX_SPLIT = 8;
 
 enum Mode : int { MODE_STORE = 0, MODE_SWIGLU = 1 };
 
@@ -54,21 +63,9 @@ struct Params {
     int* status;                     // device word: 0 ok, else the code of the wait that gave up
     long long ldq;                   // MODE_SWIGLU: bytes between rows of out
     int rows, N, E, NB, KB;          // NB, KB: blocks of 128 along N and K
+    int a_box;                       // rows of an activation copy
+    int split;                       // CTAs of a cluster, each with its part of K
     int out_bf16, accumulate, vec;   // vec: rows of out start on 16 bytes
-};
-
-template <int TILES>
-struct Cfg {
-    static constexpr int A_BYTES = BM * BK;
-    static constexpr int W_BYTES = WN * BK;
-    static constexpr int STAGE = A_BYTES + TILES * W_BYTES;
-    static constexpr int STAGES = 4;
-    static constexpr int SCALES = TILES * BM * 4;                    // bytes of a ring entry
-    static constexpr int STAGING = READERS * 1024;
-    static constexpr int BARRIERS = 2 * STAGES + 4 + 2 * RING + 1;
-    static constexpr int SMEM = STAGES * STAGE + RING * SCALES + STAGING + BARRIERS * 8 + 16 + 1024;
-    static constexpr int COLS = 32 * TILES;                          // columns a reader holds
-    static constexpr int BUF = TILES * WN;                           // tensor-memory columns of a buffer
 };
 
 __device__ __forceinline__ uint32_t instr_desc_e4m3(int m, int n) {  // e4m3 x e4m3 -> fp32, operands K-major
@@ -86,6 +83,39 @@ __device__ __forceinline__ void mma_e4m3_ss(uint32_t tmem_d, uint64_t desc_a, ui
         : "memory");
 }
 
+// The barriers of sm100.cuh by shared-memory address
+__device__ __forceinline__ bool wait_at(uint32_t bar, uint32_t parity) {
+    for (uint32_t i = 0; i < WAIT_LIMIT; ++i) {
+        uint32_t done;
+        asm volatile(
+            "{\n\t"
+            ".reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t"
+            "}"
+            : "=r"(done)
+            : "r"(bar), "r"(parity)
+            : "memory");
+        if (done) return true;
+    }
+    return false;
+}
+__device__ __forceinline__ void commit_at(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+
+__device__ __forceinline__ bool elect_one() {
+    uint32_t mine;
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t"
+        "}"
+        : "=r"(mine));
+    return mine != 0;
+}
+
 // (x, y) += (a, b) * s: the paired multiply-add, two roundings to the nearest as from two fma
 __device__ __forceinline__ void fma2(float& x, float& y, uint32_t a, uint32_t b, float s) {
     asm("{\n\t"
@@ -100,6 +130,20 @@ __device__ __forceinline__ void fma2(float& x, float& y, uint32_t a, uint32_t b,
         : "r"(a), "r"(b), "f"(s));
 }
 
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// 16 bytes of the shared memory of the cluster's CTA `rank`, at the address that `here` has in this CTA's
+__device__ __forceinline__ float4 peer_float4(uint32_t here, int rank) {
+    uint32_t at;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(here), "r"(rank));
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
+    return v;
+}
+
 // silu(g) * u with the exponential and the reciprocal as single instructions (relative error about 2^-21, before a
 // rounding to 2^-4); a large negative g gives -0 * u.
 __device__ __forceinline__ float silu_mul(float g, float u) {
@@ -108,69 +152,73 @@ __device__ __forceinline__ float silu_mul(float g, float u) {
 
 struct Tile {
     int group;                       // -1: no more tiles
-    int row0, row_end, nt;           // rows, index of the weight tile (pair)
+    int row0, rows, nt;              // its rows, index of its pair of weight tiles
 };
 
-// The tiles of a launch in order: group after group, in a group weight tile after weight tile, in those the row tiles.
-// A warp asks for tiles in ascending order; lane l holds the bounds of group base + l.
-struct Walk {
-    int base, start, end, first, count, before;
-
-    __device__ __forceinline__ void load(const Params& p, int n_tiles) {
-        const int lane = threadIdx.x & 31, e = base + lane;
-        start = end = 0;
-        if (e < p.E) {
-            start = p.group_offsets ? min(max(p.group_offsets[e], 0), p.rows) : 0;
-            end = p.group_offsets ? min(p.group_offsets[e + 1], p.rows) : p.rows;
+// Tile t of a launch: group after group, in a group weight tile after weight tile, in those the row tiles.  A warp looks it up
+// together: lane l counts the tiles of group base + l.  Nothing is kept from one tile to the next: the readers' registers
+// are full.
+__device__ __forceinline__ Tile find_tile(int t, const Params& p, int n_tiles) {
+    const int lane = threadIdx.x & 31;
+    Tile r;
+    r.group = -1;
+    r.row0 = r.rows = r.nt = 0;
+    int before = 0;
+    for (int base = 0; base < p.E; base += 32) {
+        int start = 0, end = 0;
+        if (base + lane < p.E) {
+            start = p.group_offsets ? min(max(p.group_offsets[base + lane], 0), p.rows) : 0;
+            end = p.group_offsets ? min(p.group_offsets[base + lane + 1], p.rows) : p.rows;
         }
-        count = end > start ? (end - start + BM - 1) / BM * n_tiles : 0;
+        const int count = end > start ? (end - start + BM - 1) / BM * n_tiles : 0;
         int incl = count;
+        if (p.E > 1) {
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int v = __shfl_up_sync(0xffffffffu, incl, o);
-            if (lane >= o) incl += v;
+            for (int o = 1; o < 32; o <<= 1) {
+                const int v = __shfl_up_sync(0xffffffffu, incl, o);
+                if (lane >= o) incl += v;
+            }
         }
-        first = before + incl - count;
-        before += __shfl_sync(0xffffffffu, incl, 31);
-    }
-    __device__ __forceinline__ void begin(const Params& p, int n_tiles) {
-        base = before = 0;
-        load(p, n_tiles);
-    }
-    __device__ __forceinline__ Tile at(int t, const Params& p, int n_tiles) {
-        while (t >= before && base + 32 < p.E) {
-            base += 32;
-            load(p, n_tiles);
-        }
+        const int first = before + incl - count;
         const unsigned hit = __ballot_sync(0xffffffffu, t >= first && t < first + count);
-        Tile r;
-        r.group = -1;
-        r.row0 = r.row_end = r.nt = 0;
         if (hit) {
             const int src = __ffs(hit) - 1;
             const int s = __shfl_sync(0xffffffffu, start, src), f = __shfl_sync(0xffffffffu, first, src);
-            r.row_end = __shfl_sync(0xffffffffu, end, src);
-            const int row_tiles = (r.row_end - s + BM - 1) / BM;
+            const int rows = __shfl_sync(0xffffffffu, end, src) - s;
+            const int row_tiles = (rows + BM - 1) / BM;
             r.group = base + src;
             r.nt = (t - f) / row_tiles;
-            r.row0 = s + (t - f - r.nt * row_tiles) * BM;
+            const int at = (t - f - r.nt * row_tiles) * BM;
+            r.row0 = s + at;
+            r.rows = min(BM, rows - at);
+            break;
         }
-        return r;
+        before += __shfl_sync(0xffffffffu, incl, 31);
     }
-};
+    return r;
+}
 
-template <int MODE, int TILES>
+// One output element's value and place (MODE_STORE)
+__device__ __forceinline__ void put(const Params& p, size_t at, float v) {
+    if (p.out_bf16) static_cast<bf16*>(p.out)[at] = __float2bfloat16_rn(v);
+    else if (p.accumulate) atomicAdd(static_cast<float*>(p.out) + at, v);     // one addend an element from this launch
+    else static_cast<float*>(p.out)[at] = v;
+}
+
+__device__ __forceinline__ float row_factor(const Params& p, int row) {
+    return p.row_scale ? p.row_scale[p.scale_rows ? p.scale_rows[row] : row] : 1.0f;
+}
+
+template <int MODE, bool SPLIT>
 __global__ void __launch_bounds__(THREADS, 1)
 fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w, const Params p) {
-    using C = Cfg<TILES>;
-    static_assert(MODE == MODE_STORE || TILES == 2, "gate and up are two tiles");
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    float* ring = reinterpret_cast<float*>(smem + C::STAGES * C::STAGE);                  // [RING][TILES][BM]
-    uint8_t* staging = smem + C::STAGES * C::STAGE + RING * C::SCALES;
-    uint64_t* full = reinterpret_cast<uint64_t*>(staging + C::STAGING);
-    uint64_t* empty = full + C::STAGES;
-    uint64_t* acc_full = empty + C::STAGES;
+    float* ring = reinterpret_cast<float*>(smem + STAGES * STAGE);                        // [RING][2][BM]
+    uint8_t* staging = reinterpret_cast<uint8_t*>(ring + RING * 2 * BM);
+    uint64_t* full = reinterpret_cast<uint64_t*>(staging + STAGING);
+    uint64_t* empty = full + STAGES;
+    uint64_t* acc_full = empty + STAGES;
     uint64_t* acc_empty = acc_full + 2;
     uint64_t* sc_full = acc_empty + 2;
     uint64_t* sc_empty = sc_full + RING;
@@ -178,10 +226,14 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
     uint32_t* slot = reinterpret_cast<uint32_t*>(drained + 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int I = p.N / 2;
-    const int n_tiles = MODE == MODE_SWIGLU ? I / WN : (p.N + C::BUF - 1) / C::BUF;
+    const int n_tiles = MODE == MODE_SWIGLU ? I / WN : (p.N + BN - 1) / BN;
+    // this CTA's tiles and its part of K
+    const int rank = SPLIT ? blockIdx.x % p.split : 0;
+    const int t_first = SPLIT ? blockIdx.x / p.split : blockIdx.x, t_step = SPLIT ? 0x40000000 : gridDim.x;
+    const int kb0 = SPLIT ? p.KB * rank / p.split : 0, kb1 = SPLIT ? p.KB * (rank + 1) / p.split : p.KB;
 
     if (threadIdx.x == 0) {
-        for (int s = 0; s < C::STAGES; ++s) {
+        for (int s = 0; s < STAGES; ++s) {
             mbar_init(&full[s], 1);
             mbar_init(&empty[s], 1);
         }
@@ -196,8 +248,12 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
         mbar_init(drained, 1);
         fence_barrier_init();
     }
+    if (warp == READERS) {
+        prefetch_tensormap(&map_w);
+        prefetch_tensormap(&map_a);
+    }
     if (warp == READERS + 1) {
-        tmem_alloc(slot, 2 * C::BUF);
+        tmem_alloc(slot, 2 * BN);
         tmem_relinquish();
     }
     tcgen05_fence_before();
@@ -206,133 +262,140 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
     const uint32_t tmem = *slot;
     pdl_wait();
 
-    Walk walk;
+    Tile only = {-1, 0, 0, 0};                                        // SPLIT: the cluster's tile
     if (warp >= READERS) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 32;");
-        walk.begin(p, n_tiles);
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
         int it = 0;                                                   // blocks of K so far, over all tiles
         bool ok = true;
         if (warp == READERS) {
             // ---- copies ----------------------------------------------------------------------
-            for (int t = blockIdx.x; ok; t += gridDim.x) {
-                const Tile tile = walk.at(t, p, n_tiles);
+            for (int t = t_first; ok; t += t_step) {
+                const Tile tile = find_tile(t, p, n_tiles);
                 if (tile.group < 0) break;
-                const int n0 = tile.nt * (MODE == MODE_SWIGLU ? WN : C::BUF), n1 = MODE == MODE_SWIGLU ? I + n0 : n0 + WN;
-                const int boxes = (min(BM, tile.row_end - tile.row0) + A_BOX - 1) / A_BOX;
+                const int n0 = tile.nt * (MODE == MODE_SWIGLU ? WN : BN), n1 = MODE == MODE_SWIGLU ? I + n0 : n0 + WN;
+                const int boxes = (tile.rows + p.a_box - 1) / p.a_box;
                 if (lane == 0) {
-                    for (int kb = 0; kb < p.KB; ++kb, ++it) {
-                        const int s = it % C::STAGES;
-                        if (it >= C::STAGES) ok = mbar_wait(&empty[s], (it / C::STAGES - 1) & 1);
+                    for (int kb = kb0; kb < kb1; ++kb, ++it) {
+                        const int s = it % STAGES;
+                        if (it >= STAGES) ok = mbar_wait(&empty[s], (it / STAGES - 1) & 1);
                         if (!ok) { atomicExch(p.status, 1); break; }
-                        uint8_t* stage = smem + s * C::STAGE;
-                        mbar_arrive_expect_tx(&full[s], boxes * (A_BOX * BK) + TILES * C::W_BYTES);
-                        tma_load_3d(stage + C::A_BYTES, &map_w, &full[s], kb * BK, n0, tile.group);
-                        if (TILES == 2) tma_load_3d(stage + C::A_BYTES + C::W_BYTES, &map_w, &full[s], kb * BK, n1, tile.group);
-                        for (int b = 0; b < boxes; ++b)
-                            tma_load_2d(stage + b * (A_BOX * BK), &map_a, &full[s], kb * BK, tile.row0 + b * A_BOX);
+                        uint8_t* stage = smem + s * STAGE;
+                        mbar_arrive_expect_tx(&full[s], boxes * p.a_box * BK + 2 * W_BYTES);
+                        tma_load_3d(stage + A_BYTES, &map_w, &full[s], kb * BK, n0, tile.group);
+                        tma_load_3d(stage + A_BYTES + W_BYTES, &map_w, &full[s], kb * BK, n1, tile.group);
+                        // rows of the tile only (its other lanes hold what was there; nobody reads them)
+                        for (int b = 0; b < boxes; ++b) tma_load_2d(stage + b * p.a_box * BK, &map_a, &full[s], kb * BK, tile.row0 + b * p.a_box);
                     }
                 }
                 ok = __shfl_sync(0xffffffffu, (int)ok, 0);
             }
             if (!ok && lane == 0)                                     // let the copies that were started land
-                for (int i = max(0, it - C::STAGES); i < it; ++i) mbar_wait(&full[i % C::STAGES], (i / C::STAGES) & 1, 1u << 16);
+                for (int i = max(0, it - STAGES); i < it; ++i) mbar_wait(&full[i % STAGES], (i / STAGES) & 1, 1u << 16);
         } else if (warp == READERS + 1) {
-            // ---- MMAs ------------------------------------------------------------------------
-            const uint32_t idesc = instr_desc_e4m3(BM, C::BUF);
-            for (int t = blockIdx.x; ok; t += gridDim.x) {
-                const Tile tile = walk.at(t, p, n_tiles);
+            // ---- MMAs: the whole warp walks (its counters and addresses are uniform), one thread issues ----------------
+            const uint32_t idesc = instr_desc_e4m3(BM, BN);
+            const uint64_t desc0 = smem_desc_k_sw128(smem);
+            const uint32_t full0 = smem_u32(full), empty0 = smem_u32(empty), got0 = smem_u32(acc_full), free0 = smem_u32(acc_empty);
+            for (int t = t_first; ok; t += t_step) {
+                const Tile tile = find_tile(t, p, n_tiles);
                 if (tile.group < 0) break;
-                if (lane == 0) {
-                    for (int kb = 0; kb < p.KB; ++kb, ++it) {
-                        const int s = it % C::STAGES, b = it & 1;
-                        if (it >= 2) ok = mbar_wait(&acc_empty[b], (it / 2 - 1) & 1);
-                        if (!ok) { atomicExch(p.status, 7); break; }
-                        ok = mbar_wait(&full[s], (it / C::STAGES) & 1);
-                        if (!ok) { atomicExch(p.status, 2); break; }
-                        tcgen05_fence_after();
-                        const uint8_t* stage = smem + s * C::STAGE;
+                for (int kb = kb0; kb < kb1; ++kb, ++it) {
+                    const uint32_t s = it % STAGES, b = it & 1;
+                    ok = wait_at(free0 + 8 * b, ((it >> 1) & 1) ^ 1);      // (the phase before the first counts as complete)
+                    if (!ok) { if (lane == 0) atomicExch(p.status, 7); break; }
+                    ok = wait_at(full0 + 8 * s, (it / STAGES) & 1);
+                    if (!ok) { if (lane == 0) atomicExch(p.status, 2); break; }
+                    tcgen05_fence_after();
+                    const uint64_t da = desc0 + s * (STAGE >> 4), dw = da + (A_BYTES >> 4);
+                    const uint32_t d = tmem + b * BN;
+                    if (elect_one()) {
 #pragma unroll
-                        for (int k = 0; k < BK / 32; ++k)
-                            mma_e4m3_ss(tmem + b * C::BUF, smem_desc_k_sw128(stage, k * 32), smem_desc_k_sw128(stage + C::A_BYTES, k * 32),
-                                        idesc, k != 0);
-                        mma_commit(&empty[s]);
-                        mma_commit(&acc_full[b]);
+                        for (int k = 0; k < BK / 32; ++k) mma_e4m3_ss(d, da + 2 * k, dw + 2 * k, idesc, k != 0);
+                        commit_at(empty0 + 8 * s);
+                        commit_at(got0 + 8 * b);
                     }
-                    if (!ok) {                                        // tensor memory is given back when all MMAs are done
-                        mma_commit(drained);
-                        mbar_wait(drained, 0, 1u << 16);
-                    }
+                    __syncwarp();
                 }
-                ok = __shfl_sync(0xffffffffu, (int)ok, 0);
+            }
+            if (!ok && lane == 0) {                                   // tensor memory is given back when all MMAs are done
+                mma_commit(drained);
+                mbar_wait(drained, 0, 1u << 16);
             }
         } else {
             // ---- scales: this warp the blocks of one parity --------------------------------------
-            for (int t = blockIdx.x; ok; t += gridDim.x) {
-                const Tile tile = walk.at(t, p, n_tiles);
+            for (int t = t_first; ok; t += t_step) {
+                const Tile tile = find_tile(t, p, n_tiles);
                 if (tile.group < 0) break;
-                const int nb = tile.nt * (MODE == MODE_SWIGLU ? 1 : TILES);
+                const int nb = tile.nt * (MODE == MODE_SWIGLU ? 1 : 2);
                 const float* w0 = p.w_scale + ((size_t)tile.group * p.NB + nb) * p.KB;
                 // a weight tile behind the last row of weights has no scales (its sums are not stored)
                 const float* w1 = p.w_scale + ((size_t)tile.group * p.NB + (MODE == MODE_SWIGLU ? nb + I / WN : min(nb + 1, p.NB - 1))) * p.KB;
-                const float* a[BM / 32];
-#pragma unroll
-                for (int i = 0; i < BM / 32; ++i) a[i] = p.a_scale + min(tile.row0 + i * 32 + lane, tile.row_end - 1);
+                const int last = tile.row0 + tile.rows - 1;
                 const int skip = (it ^ (warp - READERS - 2)) & 1;
-                for (int kb = skip; kb < p.KB; kb += 2) {
-                    const int i = it + kb, r = i % RING;
+                for (int kb = kb0 + skip; kb < kb1; kb += 2) {
+                    const int i = it + kb - kb0, r = i % RING;
+                    const float* a = p.a_scale + (size_t)kb * p.rows;
                     float sa[BM / 32];
 #pragma unroll
-                    for (int j = 0; j < BM / 32; ++j) sa[j] = a[j][(size_t)kb * p.rows];
-                    const float s0 = w0[kb], s1 = TILES == 2 ? w1[kb] : 0.0f;
+                    for (int j = 0; j < BM / 32; ++j) sa[j] = a[min(tile.row0 + j * 32 + lane, last)];
+                    const float s0 = w0[kb], s1 = w1[kb];
                     if (i >= RING) ok = mbar_wait(&sc_empty[r], (i / RING - 1) & 1);
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) { if (lane == 0) atomicExch(p.status, 8); break; }
 #pragma unroll
                     for (int j = 0; j < BM / 32; ++j) {
-                        float* dst = ring + r * TILES * BM + j * 32 + lane;
+                        float* dst = ring + r * 2 * BM + j * 32 + lane;
                         dst[0] = sa[j] * s0;
-                        if (TILES == 2) dst[BM] = sa[j] * s1;
+                        dst[BM] = sa[j] * s1;
                     }
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&sc_full[r]);
                 }
-                it += p.KB;
+                it += kb1 - kb0;
             }
         }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 112;");
-        // ---- readers: warp w has lanes 32 (w % 4) .. + 31 (a row a thread) and quarter w / 4 of the columns -------
-        walk.begin(p, n_tiles);
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+        // ---- readers: warp w has lanes 32 (w % 4) .. + 31 (a row a thread) and half w / 4 of the columns: a weight tile
+        // (store), or the same 64 columns of the gate's and the up tile (SwiGLU) ----------------------------------------
         const int part = warp >> 2, at = (warp & 3) * 32 + lane;
-        const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+        const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16) + part * (MODE == MODE_SWIGLU ? WN / 2 : WN);
+        constexpr int SECOND = MODE == MODE_SWIGLU ? WN : WN / 2;     // from this thread's first 64 columns to its others
         int it = 0, turn = 0;
         bool ok = true;
-        for (int t = blockIdx.x; ok; t += gridDim.x, ++turn) {
-            const Tile tile = walk.at(t, p, n_tiles);
+        for (int t = t_first; ok; t += t_step, turn ^= 1) {
+            const Tile tile = find_tile(t, p, n_tiles);
             if (tile.group < 0) break;
             const int row = tile.row0 + at;
-            const bool live = row < tile.row_end;
-            float acc[C::COLS];
+            const bool live = at < tile.rows;
+            float acc[2][64];
 #pragma unroll
-            for (int i = 0; i < C::COLS; ++i) acc[i] = 0.0f;
-            for (int kb = 0; kb < p.KB; ++kb, ++it) {
+            for (int i = 0; i < 64; ++i) acc[0][i] = acc[1][i] = 0.0f;
+            const bool any = (warp & 3) * 32 < tile.rows;             // a warp without rows keeps the count alone
+            for (int kb = kb0; kb < kb1 && !any; ++kb, ++it) {
+                ok = __all_sync(0xffffffffu, mbar_wait(&acc_full[it & 1], (it / 2) & 1));
+                if (!ok) { if (lane == 0) atomicExch(p.status, 3); break; }
+                if (lane == 0) {
+                    mbar_arrive(&acc_empty[it & 1]);
+                    mbar_arrive(&sc_empty[it % RING]);
+                }
+            }
+            for (int kb = kb0; kb < kb1 && any; ++kb, ++it) {
                 const int b = it & 1, r = it % RING;
                 ok = mbar_wait(&sc_full[r], (it / RING) & 1);
-                const float* f = ring + r * TILES * BM + at;
-                // store: this part's 64 (32) columns in a run; SwiGLU: 32 of the gate's and 32 of the up tile
-                const float s0 = f[MODE == MODE_STORE && TILES == 2 ? (part >> 1) * BM : 0];
-                const float s1 = MODE == MODE_SWIGLU ? f[BM] : s0;
+                const float* f = ring + r * 2 * BM + at;
+                const float s0 = f[MODE == MODE_STORE ? part * BM : 0], s1 = MODE == MODE_SWIGLU ? f[BM] : s0;
                 ok = ok && mbar_wait(&acc_full[b], (it / 2) & 1);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) { if (lane == 0) atomicExch(p.status, 3); break; }
                 tcgen05_fence_after();
-                uint32_t v[32];
 #pragma unroll
-                for (int c = 0; c < TILES; ++c) {
-                    const int col = MODE == MODE_SWIGLU ? c * WN + part * 32 : part * C::COLS + c * 32;
-                    tmem_ld_32_nowait(lanes + b * C::BUF + col, v);
+                for (int h = 0; h < 2; ++h) {
+                    uint32_t v[2][32];
+                    tmem_ld_32_nowait(lanes + b * BN + h * SECOND, v[0]);
+                    tmem_ld_32_nowait(lanes + b * BN + h * SECOND + 32, v[1]);
                     tmem_ld_wait();
-                    if (c == TILES - 1) {                             // all read: the buffer is free
+                    if (h == 1) {                                     // all read: the buffer is free
                         tcgen05_fence_before();
                         __syncwarp();
                         if (lane == 0) {
@@ -341,38 +404,53 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
                         }
                     }
 #pragma unroll
-                    for (int i = 0; i < 32; i += 2) fma2(acc[c * 32 + i], acc[c * 32 + i + 1], v[i], v[i + 1], c == 0 ? s0 : s1);
+                    for (int i = 0; i < 64; i += 2) fma2(acc[h][i], acc[h][i + 1], v[i / 32][i % 32], v[i / 32][i % 32 + 1], h == 0 ? s0 : s1);
                 }
             }
+            if constexpr (SPLIT) {
+                // this CTA's sums, [row][256 columns] with the 16-byte pieces of a row swapped by the row's last three bits,
+                // where its stages were: every copy has landed and every MMA has read it, or the call has failed
+                only = tile;
+                if (!ok) break;
+                if (live) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int i = 0; i < 64; i += 4) {
+                            const int piece = (part * (MODE == MODE_SWIGLU ? WN / 2 : WN) + h * SECOND + i) / 4;
+                            *reinterpret_cast<float4*>(smem + at * (BN * 4) + (piece ^ (at & 7)) * 16) =
+                                make_float4(acc[h][i], acc[h][i + 1], acc[h][i + 2], acc[h][i + 3]);
+                        }
+                }
+                break;
+            }
             if (MODE == MODE_STORE && !ok) break;
-            float rs = 1.0f;
-            if (p.row_scale && live) rs = p.row_scale[p.scale_rows ? p.scale_rows[row] : row];
+            const float rs = live ? row_factor(p, row) : 0.0f;
             uint8_t* mine = staging + warp * 1024;
             if constexpr (MODE == MODE_SWIGLU) {
-                // 32 columns of h a thread; the block's maximum over the four parts
-                float* peak = reinterpret_cast<float*>(mine) + (turn & 1) * 32;
+                // 64 columns of h a thread; the block's maximum over the two parts
+                uint32_t* peak = reinterpret_cast<uint32_t*>(staging) + turn * BM * 2 + at * 2;
                 uint32_t m = 0;
 #pragma unroll
-                for (int i = 0; i < 32; ++i) {
-                    acc[i] = silu_mul(acc[i] * rs, acc[32 + i] * rs);
-                    m = max(m, fp8::abs_bits(acc[i]));
+                for (int i = 0; i < 64; ++i) {
+                    acc[0][i] = silu_mul(acc[0][i] * rs, acc[1][i] * rs);
+                    m = max(m, fp8::abs_bits(acc[0][i]));
                 }
-                peak[lane] = __uint_as_float(m);
-                ok = named_barrier_all(1 + (warp & 3), 128, ok);      // a part that gave up takes the other three along
+                peak[part] = m;
+                ok = named_barrier_all(1 + (warp & 3), 64, ok);       // a part that gave up takes the other along
                 if (!ok) break;
-#pragma unroll
-                for (int o = 0; o < 4; ++o)
-                    m = max(m, __float_as_uint(reinterpret_cast<const float*>(staging + (o * 4 + (warp & 3)) * 1024)[(turn & 1) * 32 + lane]));
+                m = max(m, peak[part ^ 1]);
                 const float s = fp8::scale_of(m), inv = 1.0f / s;
                 if (live) {
-                    uint4* dst = reinterpret_cast<uint4*>(static_cast<uint8_t*>(p.out) + (size_t)row * p.ldq + tile.nt * WN + part * 32);
+                    uint4* dst = reinterpret_cast<uint4*>(static_cast<uint8_t*>(p.out) + (size_t)row * p.ldq + tile.nt * WN + part * 64);
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
+                    for (int i = 0; i < 4; ++i) {
                         uint32_t w[4];
 #pragma unroll
-                        for (int j = 0; j < 4; ++j)
-                            w[j] = fp8::pack4(acc[i * 16 + j * 4] * inv, acc[i * 16 + j * 4 + 1] * inv, acc[i * 16 + j * 4 + 2] * inv,
-                                              acc[i * 16 + j * 4 + 3] * inv);
+                        for (int j = 0; j < 4; ++j) {
+                            const float* x = &acc[0][i * 16 + j * 4];
+                            w[j] = fp8::pack4(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
+                        }
                         dst[i] = make_uint4(w[0], w[1], w[2], w[3]);
                     }
                     if (part == 0) p.out_scale[(size_t)tile.nt * p.rows + row] = s;
@@ -380,123 +458,241 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
             } else {
                 // 32 bytes of every row at a time go through the warp's staging, so that a store writes whole sectors
                 const int to = live ? (p.out_rows ? p.out_rows[row] : row) : -1;
-                const int c0 = tile.nt * C::BUF + part * C::COLS;
-                if (p.row_scale) {
-#pragma unroll
-                    for (int i = 0; i < C::COLS; ++i) acc[i] *= rs;
-                }
-                if (p.bias) {
-#pragma unroll
-                    for (int i = 0; i < C::COLS; ++i) acc[i] += c0 + i < p.N ? p.bias[c0 + i] : 0.0f;
-                }
+                const int c0 = tile.nt * BN + part * WN;
                 const int flip = (lane >> 2) & 1;
-                auto put = [&](int piece, uint4 v) { *reinterpret_cast<uint4*>(mine + lane * 32 + ((piece ^ flip) * 16)) = v; };
-                auto get = [&](int i) {                               // 16 bytes of row i * 16 + lane / 2
+                auto put16 = [&](int piece, uint4 v) { *reinterpret_cast<uint4*>(mine + lane * 32 + ((piece ^ flip) * 16)) = v; };
+                auto get16 = [&](int i) {                             // 16 bytes of row i * 16 + lane / 2
                     const int r = i * 16 + (lane >> 1);
                     return *reinterpret_cast<const uint4*>(mine + r * 32 + (((lane & 1) ^ ((r >> 2) & 1)) * 16));
                 };
-                if (p.out_bf16) {
-                    bf16* out = static_cast<bf16*>(p.out);
 #pragma unroll
-                    for (int c = 0; c < C::COLS; c += 16) {
+                for (int h = 0; h < 2; ++h) {
+                    if (p.row_scale) {
 #pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            uint32_t w[4];
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) {
-                                const __nv_bfloat162 two = __floats2bfloat162_rn(acc[c + h * 8 + j * 2], acc[c + h * 8 + j * 2 + 1]);
-                                w[j] = *reinterpret_cast<const uint32_t*>(&two);
-                            }
-                            put(h, make_uint4(w[0], w[1], w[2], w[3]));
-                        }
-                        __syncwarp();
-#pragma unroll
-                        for (int i = 0; i < 2; ++i) {
-                            const int r = __shfl_sync(0xffffffffu, to, i * 16 + (lane >> 1));
-                            const uint4 v = get(i);
-                            const int n = c0 + c + (lane & 1) * 8;
-                            if (r < 0 || n >= p.N) continue;
-                            bf16* dst = out + (size_t)r * p.N + n;
-                            if (p.vec && n + 8 <= p.N) {
-                                *reinterpret_cast<uint4*>(dst) = v;
-                            } else {
-                                const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                                for (int j = 0; j < 8; ++j)
-                                    if (n + j < p.N) reinterpret_cast<unsigned short*>(dst)[j] = (unsigned short)(w[j / 2] >> (16 * (j & 1)));
-                            }
-                        }
-                        __syncwarp();
+                        for (int i = 0; i < 64; ++i) acc[h][i] *= rs;
                     }
-                } else {
-                    float* out = static_cast<float*>(p.out);
+                    if (p.bias) {
 #pragma unroll
-                    for (int c = 0; c < C::COLS; c += 8) {
+                        for (int i = 0; i < 64; ++i) acc[h][i] += c0 + h * 64 + i < p.N ? p.bias[c0 + h * 64 + i] : 0.0f;
+                    }
+                    if (p.out_bf16) {
+                        bf16* out = static_cast<bf16*>(p.out);
 #pragma unroll
-                        for (int h = 0; h < 2; ++h)
-                            put(h, make_uint4(__float_as_uint(acc[c + h * 4]), __float_as_uint(acc[c + h * 4 + 1]),
-                                              __float_as_uint(acc[c + h * 4 + 2]), __float_as_uint(acc[c + h * 4 + 3])));
-                        __syncwarp();
+                        for (int c = 0; c < 64; c += 16) {
 #pragma unroll
-                        for (int i = 0; i < 2; ++i) {
-                            const int r = __shfl_sync(0xffffffffu, to, i * 16 + (lane >> 1));
-                            const uint4 v = get(i);
-                            const int n = c0 + c + (lane & 1) * 4;
-                            if (r < 0 || n >= p.N) continue;
-                            float* dst = out + (size_t)r * p.N + n;
-                            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-                            if (p.accumulate) {                       // one addend an element from this launch
+                            for (int o = 0; o < 2; ++o) {
+                                uint32_t w[4];
 #pragma unroll
-                                for (int j = 0; j < 4; ++j)
-                                    if (n + j < p.N) atomicAdd(dst + j, __uint_as_float(w[j]));
-                            } else if (p.vec && n + 4 <= p.N) {
-                                *reinterpret_cast<uint4*>(dst) = v;
-                            } else {
-#pragma unroll
-                                for (int j = 0; j < 4; ++j)
-                                    if (n + j < p.N) dst[j] = __uint_as_float(w[j]);
+                                for (int j = 0; j < 4; ++j) {
+                                    const __nv_bfloat162 two = __floats2bfloat162_rn(acc[h][c + o * 8 + j * 2], acc[h][c + o * 8 + j * 2 + 1]);
+                                    w[j] = *reinterpret_cast<const uint32_t*>(&two);
+                                }
+                                put16(o, make_uint4(w[0], w[1], w[2], w[3]));
                             }
+                            __syncwarp();
+#pragma unroll
+                            for (int i = 0; i < 2; ++i) {
+                                const int r = __shfl_sync(0xffffffffu, to, i * 16 + (lane >> 1));
+                                const uint4 v = get16(i);
+                                const int n = c0 + h * 64 + c + (lane & 1) * 8;
+                                if (r < 0 || n >= p.N) continue;
+                                bf16* dst = out + (size_t)r * p.N + n;
+                                if (p.vec && n + 8 <= p.N) {
+                                    *reinterpret_cast<uint4*>(dst) = v;
+                                } else {
+                                    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                                    for (int j = 0; j < 8; ++j)
+                                        if (n + j < p.N) reinterpret_cast<unsigned short*>(dst)[j] = (unsigned short)(w[j / 2] >> (16 * (j & 1)));
+                                }
+                            }
+                            __syncwarp();
                         }
-                        __syncwarp();
+                    } else {
+                        float* out = static_cast<float*>(p.out);
+#pragma unroll
+                        for (int c = 0; c < 64; c += 8) {
+#pragma unroll
+                            for (int o = 0; o < 2; ++o) {
+                                const float* x = &acc[h][c + o * 4];
+                                put16(o, make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3])));
+                            }
+                            __syncwarp();
+#pragma unroll
+                            for (int i = 0; i < 2; ++i) {
+                                const int r = __shfl_sync(0xffffffffu, to, i * 16 + (lane >> 1));
+                                const uint4 v = get16(i);
+                                const int n = c0 + h * 64 + c + (lane & 1) * 4;
+                                if (r < 0 || n >= p.N) continue;
+                                float* dst = out + (size_t)r * p.N + n;
+                                const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+                                if (p.vec && !p.accumulate && n + 4 <= p.N) {
+                                    *reinterpret_cast<uint4*>(dst) = v;
+                                } else {
+#pragma unroll
+                                    for (int j = 0; j < 4; ++j)
+                                        if (n + j < p.N) put(p, (size_t)r * p.N + n + j, __uint_as_float(w[j]));
+                                }
+                            }
+                            __syncwarp();
+                        }
                     }
                 }
             }
         }
     }
+    if constexpr (SPLIT) {
+        cluster_sync();
+        if (warp < READERS && only.group >= 0) {
+            // a warp a row: 4 neighbouring columns a lane (of both weight tiles), the CTAs' parts in the order of K
+            const int n0 = only.nt * (MODE == MODE_SWIGLU ? WN : BN);
+            for (int c = rank + p.split * warp; c < only.rows; c += p.split * READERS) {
+                const uint32_t here = smem_u32(smem) + c * (BN * 4) + ((lane ^ (c & 7)) * 16);
+                float4 v[2] = {make_float4(0.0f, 0.0f, 0.0f, 0.0f), make_float4(0.0f, 0.0f, 0.0f, 0.0f)};
+#pragma unroll 4
+                for (int r = 0; r < p.split; ++r) {
+#pragma unroll
+                    for (int w = 0; w < 2; ++w) {
+                        const float4 x = peer_float4(here + w * WN * 4, r);
+                        v[w].x += x.x;
+                        v[w].y += x.y;
+                        v[w].z += x.z;
+                        v[w].w += x.w;
+                    }
+                }
+                const int row = only.row0 + c;
+                const float rs = row_factor(p, row);
+                if constexpr (MODE == MODE_SWIGLU) {
+                    const float h[4] = {silu_mul(v[0].x * rs, v[1].x * rs), silu_mul(v[0].y * rs, v[1].y * rs),
+                                        silu_mul(v[0].z * rs, v[1].z * rs), silu_mul(v[0].w * rs, v[1].w * rs)};
+                    uint32_t m = 0;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) m = max(m, fp8::abs_bits(h[i]));
+                    const float scale = fp8::scale_of(__reduce_max_sync(0xffffffffu, m)), inv = 1.0f / scale;
+                    *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(p.out) + (size_t)row * p.ldq + n0 + lane * 4) =
+                        fp8::pack4(h[0] * inv, h[1] * inv, h[2] * inv, h[3] * inv);
+                    if (lane == 0) p.out_scale[(size_t)only.nt * p.rows + row] = scale;
+                } else {
+                    const size_t to = p.out_rows ? p.out_rows[row] : row;
+#pragma unroll
+                    for (int w = 0; w < 2; ++w) {
+                        const int n = n0 + w * WN + lane * 4;
+                        if (n >= p.N) continue;
+                        float x[4] = {v[w].x, v[w].y, v[w].z, v[w].w};
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            if (p.row_scale) x[i] *= rs;
+                            if (p.bias) x[i] += p.bias[min(n + i, p.N - 1)];
+                        }
+                        if (p.vec && !p.accumulate) {
+                            if (p.out_bf16) store_four(static_cast<bf16*>(p.out) + to * p.N + n, x);
+                            else store_four(static_cast<float*>(p.out) + to * p.N + n, x);
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                if (n + i < p.N) put(p, to * p.N + n + i, x[i]);
+                        }
+                    }
+                }
+            }
+        }
+        cluster_sync();                                               // nobody leaves while its sums are read
+    }
     tcgen05_fence_before();
     __syncthreads();
     if (warp == READERS + 1) {
         tcgen05_fence_after();
-        tmem_dealloc(tmem, 2 * C::BUF);
+        tmem_dealloc(tmem, 2 * BN);
     }
 }
 
-template <int MODE, int TILES>
+template <int MODE, bool SPLIT>
 int launch(const CUtensorMap& ma, const CUtensorMap& mw, const Params& p, int ctas, cudaStream_t stream) {
-    const auto kernel = fp8_gemm_kernel<MODE, TILES>;
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<TILES>::SMEM) != cudaSuccess) return SHARPI_LAUNCH_FAILED;
-    SHARPI_LAUNCH_PDL(kernel, ctas, THREADS, Cfg<TILES>::SMEM, stream, ma, mw, p);
-    return SHARPI_OK;
+    const auto kernel = fp8_gemm_kernel<MODE, SPLIT>;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM) != cudaSuccess) return SHARPI_LAUNCH_FAILED;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = ctas;
+    cfg.blockDim = THREADS;
+    cfg.dynamicSmemBytes = SMEM;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    int n = 0;
+    if (SPLIT) {
+        attr[n].id = cudaLaunchAttributeClusterDimension;
+        attr[n].val.clusterDim.x = p.split;
+        attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
+        ++n;
+    }
+    if (sharpi_pdl_enabled()) {
+        attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[n].val.programmaticStreamSerializationAllowed = 1;
+        ++n;
+    }
+    cfg.attrs = attr;
+    cfg.numAttrs = n;
+    return cudaLaunchKernelEx(&cfg, kernel, ma, mw, p) == cudaSuccess ? SHARPI_OK : SHARPI_LAUNCH_FAILED;
+}
+
+// How many clusters of `split` CTAs the device holds at once (asked once a device)
+int clusters_at_once(int split) {
+    constexpr int DEVICES = 64;
+    static int known[DEVICES][MAX_SPLIT + 1];
+    int device = 0;
+    if (cudaGetDevice(&device) != cudaSuccess || device >= DEVICES) return 0;
+    if (known[device][split] == 0) {
+        const auto kernel = fp8_gemm_kernel<MODE_STORE, true>;
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = 8 * split;
+        cfg.blockDim = THREADS;
+        cfg.dynamicSmemBytes = SMEM;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = split;
+        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        int n = 0;
+        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM) != cudaSuccess ||
+            cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n <= 0)
+            n = -1;
+        known[device][split] = n;
+    }
+    return known[device][split];
+}
+
+// Into how many CTAs a tile's K is cut: the fewest blocks of K one after the other, a wave of clusters counted as its blocks
+// and what starting it and joining the parts takes.
+int choose_split(long long tiles, int KB, int sms) {
+    int best = 1;
+    long long least = (tiles + sms - 1) / sms * KB + 3;
+    for (int s = 2; s <= MAX_SPLIT && s <= KB; ++s) {
+        const int at_once = clusters_at_once(s);
+        if (at_once <= 0) continue;
+        const long long cost = (tiles + at_once - 1) / at_once * ((KB + s - 1) / s + 5);
+        if (cost < least) {
+            least = cost;
+            best = s;
+        }
+    }
+    return best;
 }
 
 }  // namespace
 
 // a [rows, K] with rows `lda` bytes apart, w [E, N, K] with rows `ldw` and groups `ldw * N` bytes apart (multiples of 16).
 // swiglu: out e4m3 with rows `ldq` bytes apart and out_scale [N / 256, rows]; else out float32 / bfloat16 [*, N].
+// split: 0 = chosen here, else into how many CTAs a tile's K is cut.
 SHARPI_API int sharpi_fp8_gemm(const void* a, long long lda, const float* a_scale, const void* w, long long ldw, const float* w_scale,
                                const int* group_offsets, const int* out_rows, const float* row_scale, const int* scale_rows,
                                const float* bias, void* out, long long ldq, float* out_scale, int* status, int rows, int N, int K,
-                               int E, int swiglu, int out_bf16, int accumulate, int sms, cudaStream_t stream) {
+                               int E, int swiglu, int out_bf16, int accumulate, int split, int sms, cudaStream_t stream) {
     if (rows <= 0 || N <= 0) return SHARPI_OK;
     if (K <= 0 || E <= 0 || (E > 1 && !group_offsets) || sms <= 0 || (swiglu && (N % 256 || ldq % 16 || !out_scale)) ||
-        (accumulate && (out_bf16 || swiglu)))
+        (accumulate && (out_bf16 || swiglu)) || split < 0 || split > MAX_SPLIT || split > (K + BK - 1) / BK)
         return SHARPI_BAD_ARGUMENT;
     if (lda % 16 || ldw % 16 || lda < K || ldw < K || ((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(w)) & 15) ||
         (swiglu && (reinterpret_cast<uintptr_t>(out) & 15)))
         return SHARPI_UNALIGNED;
-    const long long m_tiles = (rows + BM - 1) / BM + (E > 1 ? (rows < E ? rows : E) : 0);    // at most
-    CUtensorMap ma, mw;
-    if (!tmap::make_u8_map(&ma, a, K, rows, 0, lda, A_BOX) || !tmap::make_u8_map(&mw, w, K, N, E, ldw, WN)) return SHARPI_BAD_ARGUMENT;
     Params p = {};
     p.a_scale = a_scale;
     p.w_scale = w_scale;
@@ -517,9 +713,18 @@ SHARPI_API int sharpi_fp8_gemm(const void* a, long long lda, const float* a_scal
     p.out_bf16 = out_bf16;
     p.accumulate = accumulate;
     p.vec = (reinterpret_cast<uintptr_t>(out) & 15) == 0 && N % (out_bf16 ? 8 : 4) == 0;
-    const int cols = swiglu ? 128 : 256;
-    const long long tiles = m_tiles * (((swiglu ? N / 2 : N) + cols - 1) / cols);
-    if (tiles > 0x3fffffff) return SHARPI_BAD_ARGUMENT;
+    const long long row_tiles = rows < E ? rows : (rows + BM - 1) / BM + (E > 1 ? E : 0);        // at most
+    const long long tiles = row_tiles * (swiglu ? N / BN : (N + BN - 1) / BN);
+    if (tiles > 0x3fffffff / MAX_SPLIT) return SHARPI_BAD_ARGUMENT;
+    p.split = split ? split : choose_split(tiles, p.KB, sms);
+    // copies as small as a few rows, as few as many rows of one matrix allow
+    p.a_box = rows <= 16 ? 16 : E == 1 && rows > 96 ? 128 : 32;
+    CUtensorMap ma, mw;
+    if (!tmap::make_u8_map(&ma, a, K, rows, 0, lda, p.a_box) || !tmap::make_u8_map(&mw, w, K, N, E, ldw, WN)) return SHARPI_BAD_ARGUMENT;
+    if (p.split > 1) {
+        const int ctas = (int)tiles * p.split;
+        return swiglu ? launch<MODE_SWIGLU, true>(ma, mw, p, ctas, stream) : launch<MODE_STORE, true>(ma, mw, p, ctas, stream);
+    }
     const int ctas = (int)(tiles < sms ? tiles : sms);
-    return swiglu ? launch<MODE_SWIGLU, 2>(ma, mw, p, ctas, stream) : launch<MODE_STORE, 2>(ma, mw, p, ctas, stream);
+    return swiglu ? launch<MODE_SWIGLU, false>(ma, mw, p, ctas, stream) : launch<MODE_STORE, false>(ma, mw, p, ctas, stream);
 }

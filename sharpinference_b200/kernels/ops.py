@@ -2190,7 +2190,7 @@ _OUT_DTYPES = (torch.float32, torch.bfloat16)
 
 
 def _fp8_product(a, a_scale, w, w_scale, group_offsets, *, swiglu=False, out=None, out_scale=None, out_dtype=torch.float32,
-                 out_rows=None, row_scale=None, scale_rows=None, bias=None, accumulate=False):
+                 out_rows=None, row_scale=None, scale_rows=None, bias=None, accumulate=False, split=0):
     if a.dim() != 2 or w.dim() not in (2, 3) or a.shape[1] != w.shape[-1] or a.shape[1] == 0:
         raise KernelError(f"inner sizes differ or shapes are not [rows, K] and [N, K] or [E, N, K]: a {tuple(a.shape)}, w {tuple(w.shape)}")
     rows, K = a.shape
@@ -2239,7 +2239,7 @@ def _fp8_product(a, a_scale, w, w_scale, group_offsets, *, swiglu=False, out=Non
     check(kernel("sharpi_fp8_gemm")(a.data_ptr(), lda, a_scale.data_ptr(), w.data_ptr(), ldw, w_scale.data_ptr(), _ptr(group_offsets),
                                     _ptr(out_rows), _ptr(row_scale), _ptr(scale_rows), _ptr(bias), out.data_ptr(),
                                     out.stride(0) if swiglu else 0, _ptr(out_scale), status_word(a.device).data_ptr(), rows, N, K, E,
-                                    int(swiglu), int(out.dtype == torch.bfloat16), int(accumulate), sm_count(a.device), _stream()),
+                                    int(swiglu), int(out.dtype == torch.bfloat16), int(accumulate), split, sm_count(a.device), _stream()),
           "sharpi_fp8_gemm")
     return out
 

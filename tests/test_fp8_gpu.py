@@ -356,3 +356,43 @@ def test_in_a_graph_and_on_another_stream(ops):
         got, _ = mixture(ops, *case)
     side.synchronize()
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("split", [1, 2, 3, 5, 8])
+@pytest.mark.parametrize("M,N,K", [(1, 300, 1024), (37, 256, 1100), (128, 130, 1153), (200, 515, 2048)])
+def test_split_over_k(ops, split, M, N, K):
+    """Every way of cutting K over the CTAs of a cluster, whatever the sizes would choose."""
+    t = operands(ops, M, N, K, seed=M + split)
+    want, S = product(*t)
+    bias, base = rnd(N, seed=8), rnd(M, N, seed=9)
+    err = product_error(K, S) + split * 2.0 ** -24 * S
+    close(ops._fp8_product(*t, None, split=split), want, err)
+    close(ops._fp8_product(*t, None, split=split, bias=bias, out_dtype=BF16), want + bias.to(F64), err + (want.abs() + bias.abs()) * 2.0 ** -24)
+    out = base.clone()
+    ops._fp8_product(*t, None, split=split, out=out, accumulate=True)
+    close(out, want + base.to(F64), err + (want.abs() + base.abs()) * 2.0 ** -23)
+
+
+@pytest.mark.parametrize("split", [1, 3, 8])
+@pytest.mark.parametrize("name", ["empty_experts", "over_a_tile", "rows_behind"])
+def test_split_over_k_by_experts(ops, name, split):
+    offsets = torch.tensor(OFFSETS[name], dtype=torch.int32, device=DEV)
+    last, I, K, N = OFFSETS[name][-1], 256, 1030, 300
+    rows = last + (11 if name == "rows_behind" else 0)
+    at = torch.randperm(rows, generator=torch.Generator().manual_seed(3)).to(torch.int32).to(DEV)
+    weight = rnd(rows, seed=4).abs()
+    s = weight[at.long()][:last].to(F64).unsqueeze(1)
+    t = operands(ops, rows, 2 * I, K, E=4, seed=I + rows)
+    q, scale = ops.fp8_empty((rows, I), DEV), torch.empty(blocks(I), rows, device=DEV)
+    ops._fp8_product(*t, offsets, swiglu=True, out=q, out_scale=scale, row_scale=weight, scale_rows=at, split=split)
+    C, S = product(*t, offsets)
+    check_swiglu(q[:last], scale[:, :last], C[:last], S[:last] * (1 + split * 2.0 ** -9), K, s)
+    t = operands(ops, rows, N, K, E=4, seed=rows)
+    C, S = product(*t, offsets)
+    out = torch.full((rows, N), 5.0, device=DEV)
+    ops._fp8_product(*t, offsets, out=out, out_rows=at, row_scale=weight, scale_rows=at, split=split)
+    there = at[:last].long()
+    close(out[there], C[:last] * s, (product_error(K, S)[:last] + split * 2.0 ** -24 * S[:last] + C[:last].abs() * 2.0 ** -24) * s)
+    left = torch.ones(rows, dtype=torch.bool, device=DEV)
+    left[there] = False
+    assert (out[left] == 5.0).all()
