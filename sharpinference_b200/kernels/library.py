@@ -107,7 +107,7 @@ SIGNATURES: Dict[str, Tuple[str, list]] = {
     "sharpi_fp8_rows": ("fp8_quant", [P, I, LL, P, I, I, P, LL, P, P]),
     "sharpi_fp8_weight": ("fp8_quant", [P, I, I, I, I, LL, LL, P, LL, P, P]),
     "sharpi_fp8_gemm": ("fp8_gemm", [P, LL, P, P, LL, P, P, P, P, P, P, P, LL, P, P, I, I, I, I, I, I, I, I, I, P]),
-    "sharpi_moe_few": ("moe_few", [P, I, I, P, I, P, P, P, P, LL, P, P, LL, P, P, P, P, P, P, P, I, I, I, I, I, I, I, I, F, I, I, P]),
+    "sharpi_moe_few": ("moe_few", [P, I, I, P, I, P, P, P, P, LL, P, P, LL, P, P, P, P, P, I, I, I, I, I, I, I, I, F, I, I, P]),
     "sharpi_gated_group_norm": ("mamba2", [P, P, I, P, F, I, I, I, P, I, P]),
 }
 

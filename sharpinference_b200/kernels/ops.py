@@ -2371,18 +2371,14 @@ def moe_few(h: torch.Tensor, router_weight: torch.Tensor, gate_up: torch.Tensor,
     _here(h, router_weight, gate_up, down, h32, gate_up_scale, down_scale, correction, bias, add, out)
     if T == 0:
         return out
-    if H % 16 and w8:                     # rows of whole 16-element pieces, zeros behind the end
-        rows = torch.nn.functional.pad(h, (0, -H % 16))
-    else:
-        rows = h
-    x = rows if h32 is None else h32
-    act = min(E, T * k) * T * ((I + 15) // 16 * 16) * 2
-    work = torch.empty(act + 4 * T * E + 4, dtype=torch.uint8, device=h.device)       # act, logits, the barrier's counter
-    at = work.data_ptr()
-    check(kernel("sharpi_moe_few")(x.data_ptr(), dtype_code(x.dtype), x.shape[1], rows.data_ptr(), rows.shape[1], router_weight.data_ptr(),
-                                   _ptr(bias), _ptr(correction), gate_up.data_ptr(), ldg, _ptr(gate_up_scale), down.data_ptr(), ldd,
-                                   _ptr(down_scale), _ptr(add), at + act, at, at + act + 4 * T * E, status_word(h.device).data_ptr(),
-                                   out.data_ptr(), int(out.dtype == torch.bfloat16), T, E, k, H, I, ROUTER_SCORING[scoring],
-                                   int(renormalize), float(scale), int(weights_on == "input"), sm_count(h.device), _stream()),
-          "sharpi_moe_few")
+    x = h if h32 is None else h32
+    # the router's logits, silu(g) u of every (expert, token), the barrier's counters; with 8-bit weights activations in pieces
+    slots, inner, wide = min(E, T * k), fp8_blocks(I) * FP8_BLOCK, fp8_blocks(H)
+    size = 64 + 4 * T * E + slots * T * inner * (6 if w8 else 2) + (4 * slots * T * (inner // FP8_BLOCK) + T * wide * (2 * FP8_BLOCK + 4) if w8 else 0) + 96
+    work = torch.empty(size, dtype=torch.uint8, device=h.device)
+    check(kernel("sharpi_moe_few")(x.data_ptr(), dtype_code(x.dtype), H, h.data_ptr(), H, router_weight.data_ptr(), _ptr(bias),
+                                   _ptr(correction), gate_up.data_ptr(), ldg, _ptr(gate_up_scale), down.data_ptr(), ldd, _ptr(down_scale),
+                                   _ptr(add), work.data_ptr(), status_word(h.device).data_ptr(), out.data_ptr(),
+                                   int(out.dtype == torch.bfloat16), T, E, k, H, I, ROUTER_SCORING[scoring], int(renormalize),
+                                   float(scale), int(weights_on == "input"), sm_count(h.device), _stream()), "sharpi_moe_few")
     return out

@@ -150,6 +150,19 @@ def test_weights_whose_rows_lie_apart(ops):
     assert torch.equal(call(ops, dict(c, gate_up=wide[..., :H]), k), want)
 
 
+@pytest.mark.parametrize("H,I", [(257, 130), (128, 64)])
+def test_what_lies_between_rows_of_8_bit_weights_is_not_read(ops, H, I):
+    T, E, k = 5, 6, 2
+    c = layer(ops, T, E, H, I, "e4m3", seed=12)
+    want = call(ops, c, k)
+    for name in ("gate_up", "down"):
+        n, m = c[name].shape[1:]
+        wide = torch.full((E, n, (m + 15) // 16 * 16 + 32), 0x7f, dtype=torch.uint8, device=DEV)       # e4m3's NaN
+        wide[..., :m] = c[name].view(torch.uint8) if c[name].is_contiguous() else c[name].contiguous().view(torch.uint8)
+        c[name] = wide.view(torch.float8_e4m3fn)[..., :m]
+    assert torch.equal(call(ops, c, k), want)
+
+
 @pytest.mark.parametrize("weights", ["bfloat16", "e4m3"])
 def test_the_same_again_in_graphs_and_on_streams(ops, weights):
     T, E, H, I, k = 6, 32, 512, 256, 4
