@@ -7,11 +7,13 @@
 // With few tokens the layer is a stream of the chosen experts' weights, so the second kernel is laid out for that alone: one
 // CTA an SM, weight rows dealt out evenly over the warps whatever expert they belong to, each weight read once, in 16-byte
 // pieces straight into registers.  Teams of 1 to 16 warps share K in turn (the more K has, the more); a warp asks for its next
-// step of up to 4 KB when it has multiplied the last (up to 64 KB an SM in flight; reading at 6.4 TB/s with a microsecond of
-// latency takes 44 KB).  All tokens are the 16-row operand of the MMA against tiles of eight weight rows; a row of a token that did not choose the expert is computed and dropped (gate|up) or
-// zero (down).  Because the down product is linear, a token's experts are one long sum over (expert, inner element): act is
-// multiplied by the router's weight before (weights on the output).  The warps' parts are added in warp order: a call's result
-// is the same every time, but the order (float32 rounding) of a token's sum goes by which experts the whole call reaches.
+// step of 4 KB when it has multiplied the last (up to 64 KB an SM in flight; reading at 6.4 TB/s with a microsecond of latency
+// takes 44 KB), and rows are asked into L2 before that.  Weights are the 16-row operand of the MMA (eight gate rows and their up
+// rows, or sixteen rows of the down matrix), tokens the eight columns; a column of a token that did not choose the expert is
+// computed and dropped (gate|up) or zero (down).  Because the down product is linear, a token's experts are one long sum over
+// (expert, inner element): act is multiplied by the router's weight before (weights on the output).  The warps' parts are added
+// in warp order: a call's result is the same every time, but the order (float32 rounding) of a token's sum goes by which
+// experts the whole call reaches.
 //
 // bfloat16 weights: mma.sync m16n8k16, act rounded to bfloat16 (2^-9 of its value) as in the other bfloat16 mixtures.
 //
@@ -30,7 +32,7 @@ namespace {
 
 constexpr int MAX_T = 16, MAX_K = 32, MAX_E = 1024;
 constexpr int WARPS = 16, THREADS = 32 * WARPS;
-constexpr int NT = 4;                          // tiles of eight weight rows that a warp has at a time
+constexpr int NT = 2;                          // tiles of sixteen weight rows that a warp has at a time
 constexpr uint32_t BARRIER_LIMIT = 1u << 22;
 
 struct Params {
@@ -70,6 +72,12 @@ __device__ __forceinline__ uint2 halves(const float (&v)[4], float s) {
     return make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
 }
 
+// Memory into L2, ahead of the loads: rows whose reads would wait for a step each then wait for L2 alone.  (Nothing is read by
+// it, so it may run ahead of whoever writes there.)
+__device__ __forceinline__ void ask_for(const void* p, unsigned bytes) {
+    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"(bytes) : "memory");
+}
+
 // One warp a (token, expert), the additions in the order of the router kernels for more tokens: lane l adds the elements
 // 128 i + 4 l + u in ascending i into chain u, the chains and then the lanes are added in a fixed order.
 template <typename T>
@@ -78,6 +86,7 @@ moe_few_router_kernel(const T* h, int ldh, const float* wr, int tokens, int H, i
                       const bf16* rows, int ld_rows, __half* rows16, int ld16, float* x_scale) {
     const int item = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
     const int e = item / tokens, t = item - e * tokens;
+    if (vec && t == 0 && e < E && lane == 0) ask_for(wr + (size_t)e * H, H * 4);
     pdl_wait();
     if (blockIdx.x == 0 && threadIdx.x < 2) barrier[threadIdx.x] = 0;
     if (e >= E) {                                        // e4m3 weights: the warps behind the experts' make h float16
@@ -99,22 +108,33 @@ moe_few_router_kernel(const T* h, int ldh, const float* wr, int tokens, int H, i
     const float* w = wr + (size_t)e * H;
     float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     if (vec) {
-#pragma unroll 8
-        for (int i = 4 * lane; i < H; i += 128) {
-            const float4 wv = *reinterpret_cast<const float4*>(w + i);
-            float xv[4];
-            if constexpr (sizeof(T) == 4) {
-                const float4 q = *reinterpret_cast<const float4*>(x + i);
-                xv[0] = q.x; xv[1] = q.y; xv[2] = q.z; xv[3] = q.w;
-            } else {
-                const uint2 q = *reinterpret_cast<const uint2*>(x + i);
-                xv[0] = __uint_as_float(q.x << 16); xv[1] = __uint_as_float(q.x & 0xffff0000u);
-                xv[2] = __uint_as_float(q.y << 16); xv[3] = __uint_as_float(q.y & 0xffff0000u);
+        constexpr int BATCH = 8;                         // loads in flight, whatever is left of the row
+#pragma unroll 1
+        for (int i0 = 4 * lane; i0 < H; i0 += 128 * BATCH) {
+            float4 wv[BATCH];
+            float xv[BATCH][4];
+#pragma unroll
+            for (int b = 0; b < BATCH; ++b) {
+                const int i = i0 + 128 * b;
+                if (i >= H) continue;
+                wv[b] = *reinterpret_cast<const float4*>(w + i);
+                if constexpr (sizeof(T) == 4) {
+                    const float4 q = *reinterpret_cast<const float4*>(x + i);
+                    xv[b][0] = q.x; xv[b][1] = q.y; xv[b][2] = q.z; xv[b][3] = q.w;
+                } else {
+                    const uint2 q = *reinterpret_cast<const uint2*>(x + i);
+                    xv[b][0] = __uint_as_float(q.x << 16); xv[b][1] = __uint_as_float(q.x & 0xffff0000u);
+                    xv[b][2] = __uint_as_float(q.y << 16); xv[b][3] = __uint_as_float(q.y & 0xffff0000u);
+                }
             }
-            acc[0] = fmaf(xv[0], wv.x, acc[0]);
-            acc[1] = fmaf(xv[1], wv.y, acc[1]);
-            acc[2] = fmaf(xv[2], wv.z, acc[2]);
-            acc[3] = fmaf(xv[3], wv.w, acc[3]);
+#pragma unroll
+            for (int b = 0; b < BATCH; ++b) {
+                if (i0 + 128 * b >= H) continue;
+                acc[0] = fmaf(xv[b][0], wv[b].x, acc[0]);
+                acc[1] = fmaf(xv[b][1], wv[b].y, acc[1]);
+                acc[2] = fmaf(xv[b][2], wv[b].z, acc[2]);
+                acc[3] = fmaf(xv[b][3], wv[b].w, acc[3]);
+            }
         }
     } else {
         for (int i = 4 * lane; i < H; i += 128) {
@@ -152,8 +172,9 @@ __device__ __forceinline__ void widen(uint32_t w, uint32_t& lo, uint32_t& hi) {
         : "r"(w));
 }
 
-// How a step of a warp reads K: a lane has 16 bytes of a weight row in each of two pieces; lanes 4 g + t of a row lie side
-// by side.  Which elements of K share an MMA is free as long as both operands agree: lane t's elements are its k values.
+// How a step of a warp reads K: a lane has 16 bytes of two weight rows (eight apart in the tile) in each of two pieces; lanes
+// 4 g + t of a row lie side by side.  Which elements of K share an MMA is free as long as both operands agree: lane t's
+// elements are its k values.
 constexpr int STEP = 128;         // bytes of a row: one block of e4m3, 64 bfloat16 values
 
 // The first `left` of 16 bytes, zeros behind them
@@ -167,80 +188,106 @@ __device__ __forceinline__ uint4 cut(uint4 v, int left) {
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// The weights of a step of a warp; `row`: this lane's row of every tile (where a tile has none, any row: its sums are
-// dropped), `tiles` of which are read; `len`: bytes of a row.
-__device__ __forceinline__ void fetch(uint4 (&w)[NT][2], const uint8_t* const (&row)[NT], int tiles, int at, int len) {
+// A tile's weights of a step: [row g or g + 8][piece].  `len`: bytes of a row; behind them zeros, whatever lies between rows.
+__device__ __forceinline__ void fetch(uint4 (&w)[2][2], const uint8_t* low, const uint8_t* high, int at, int len) {
     const int k = at + (threadIdx.x & 3) * 16;
     if (at + STEP <= len) {
+        w[0][0] = load_stream(low + k);
+        w[1][0] = load_stream(high + k);
+        w[0][1] = load_stream(low + k + 64);
+        w[1][1] = load_stream(high + k + 64);
+    } else {
 #pragma unroll
-        for (int i = 0; i < NT; ++i)
-            if (i < tiles) {
-                w[i][0] = load_stream(row[i] + k);
-                w[i][1] = load_stream(row[i] + k + 64);
-            }
-    } else {                                                              // behind the end: zeros, whatever lies between rows
-#pragma unroll
-        for (int i = 0; i < NT; ++i)
-#pragma unroll
-            for (int p = 0; p < 2; ++p) {
-                const int left = len - (k + 64 * p);
-                w[i][p] = i < tiles && left > 0 ? cut(load_stream(row[i] + k + 64 * p), left) : make_uint4(0u, 0u, 0u, 0u);
-            }
+        for (int p = 0; p < 2; ++p) {
+            const int left = len - (k + 64 * p);
+            w[0][p] = left > 0 ? cut(load_stream(low + k + 64 * p), left) : make_uint4(0u, 0u, 0u, 0u);
+            w[1][p] = left > 0 ? cut(load_stream(high + k + 64 * p), left) : make_uint4(0u, 0u, 0u, 0u);
+        }
     }
 }
 
-// acc += the step's products.  lo / hi: this lane's token row (and the row eight below) at the step's first element, null:
-// zeros; e4m3: `f_lo`, `f_hi`: scales of the token rows' block, scale[i]: of the block of this lane's two sums of tile i.
-// left: bytes from the step's first to the end of the (zero-padded) token rows.
-template <bool W8, bool WIDE>
-__device__ __forceinline__ void multiply(float (&acc)[NT][4], const uint4 (&w)[NT][2], int tiles, const uint8_t* lo, const uint8_t* hi, int left,
-                                         float f_lo, float f_hi, const float (&scale)[NT]) {
-    constexpr int PARTS = W8 ? 2 : 1;                                     // 16-byte parts of a lane's elements of a token row
-    const int k = (threadIdx.x & 3) * (16 * PARTS);
-    const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
-    float part[NT][4];
+// Eight tokens' elements of a step: [piece][16-byte parts of a lane's elements of its token's row].  `left`: bytes of the row
+// from here on.
+template <bool W8>
+struct Tokens {
+    static constexpr int PARTS = W8 ? 2 : 1;
+    uint4 v[2][PARTS];
+    __device__ __forceinline__ void load(const uint8_t* row, int left) {
+        const int k = (threadIdx.x & 3) * (16 * PARTS);
+        if (left >= 2 * 64 * PARTS) {
 #pragma unroll
-    for (int i = 0; i < NT; ++i)
+            for (int p = 0; p < 2; ++p)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) part[i][j] = W8 ? 0.0f : acc[i][j];
+                for (int q = 0; q < PARTS; ++q) v[p][q] = *reinterpret_cast<const uint4*>(row + k + 64 * PARTS * p + 16 * q);
+        } else {
+#pragma unroll
+            for (int p = 0; p < 2; ++p)
+#pragma unroll
+                for (int q = 0; q < PARTS; ++q) {
+                    const int at = k + 64 * PARTS * p + 16 * q;
+                    v[p][q] = at < left ? *reinterpret_cast<const uint4*>(row + at) : make_uint4(0u, 0u, 0u, 0u);
+                }
+        }
+    }
+};
+
+// sums[n][4] += a tile's products with the tokens 8 n .. + 7: rows g (elements 0, 1) and g + 8 (2, 3) by tokens 2 t and 2 t + 1
+template <bool W8, int COLS>
+__device__ __forceinline__ void multiply(float (&sums)[COLS][4], const uint4 (&w)[2][2], const Tokens<W8> (&x)[COLS]) {
 #pragma unroll
     for (int p = 0; p < 2; ++p) {
-        const int at = k + p * 64 * PARTS;
-        const bool in = at < left;
+        const uint32_t low[4] = {w[0][p].x, w[0][p].y, w[0][p].z, w[0][p].w}, high[4] = {w[1][p].x, w[1][p].y, w[1][p].z, w[1][p].w};
 #pragma unroll
-        for (int q = 0; q < PARTS; ++q) {
-            const uint4 l = lo && in ? *reinterpret_cast<const uint4*>(lo + at + 16 * q) : zero;
-            const uint4 h = WIDE && hi && in ? *reinterpret_cast<const uint4*>(hi + at + 16 * q) : zero;
-            const uint32_t a0[4] = {l.x, h.x, l.y, h.y}, a1[4] = {l.z, h.z, l.w, h.w};
-            // the tiles in turn: a product that adds to what the one before it left waits for that
+        for (int j = 0; j < (W8 ? 4 : 2); ++j) {
+            uint32_t a[4];
+            if constexpr (W8) {
+                widen(low[j], a[0], a[2]);
+                widen(high[j], a[1], a[3]);
+            } else {
+                a[0] = low[2 * j];
+                a[1] = high[2 * j];
+                a[2] = low[2 * j + 1];
+                a[3] = high[2 * j + 1];
+            }
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const uint32_t (&a)[4] = j ? a1 : a0;
-#pragma unroll
-                for (int i = 0; i < NT; ++i) {
-                    if (i >= tiles) continue;
-                    if constexpr (W8) {
-                        const uint32_t word = q ? (j ? w[i][p].w : w[i][p].z) : (j ? w[i][p].y : w[i][p].x);
-                        uint32_t b0, b1;
-                        widen(word, b0, b1);
-                        mma_f16(part[i], a, b0, b1);
-                    } else {
-                        mma16::mma_bf16(part[i], a, j ? w[i][p].z : w[i][p].x, j ? w[i][p].w : w[i][p].y);
-                    }
-                }
+            for (int n = 0; n < COLS; ++n) {
+                const uint4 v = x[n].v[p][W8 ? j / 2 : 0];
+                const uint32_t b0 = j % 2 ? v.z : v.x, b1 = j % 2 ? v.w : v.y;
+                if constexpr (W8) mma_f16(sums[n], a, b0, b1);
+                else mma16::mma_bf16(sums[n], a, b0, b1);
             }
         }
     }
+}
+
+// What a block's products are multiplied by (e4m3): the scales of rows g and g + 8 and of tokens 2 t and 2 t + 1
+template <int COLS>
+struct Factors {
+    float row[2], token[COLS][2];
+};
+
+// The same with a block's sums scaled before they are added (e4m3)
+template <bool W8, int COLS>
+__device__ __forceinline__ void accumulate(float (&acc)[COLS][4], const uint4 (&w)[2][2], const Tokens<W8> (&x)[COLS], const Factors<COLS>& f) {
+    if constexpr (W8) {
+        float part[COLS][4];
 #pragma unroll
-    for (int i = 0; i < NT; ++i) {
-        const float s_lo = scale[i] * f_lo, s_hi = scale[i] * f_hi;
+        for (int n = 0; n < COLS; ++n)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = W8 ? fmaf(part[i][j], j < 2 ? s_lo : s_hi, acc[i][j]) : part[i][j];
+            for (int j = 0; j < 4; ++j) part[n][j] = 0.0f;
+        multiply<W8, COLS>(part, w, x);
+#pragma unroll
+        for (int n = 0; n < COLS; ++n)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[n][j] = fmaf(part[n][j], f.row[j / 2] * f.token[n][j % 2], acc[n][j]);
+    } else {
+        multiply<W8, COLS>(acc, w, x);
     }
 }
 
 struct alignas(16) Shared {
-    float part[WARPS][NT][2][MAX_T][4];      // [warp][tile][half of its eight rows][token][row]
+    float4 part[WARPS][NT][MAX_T / 8][32];   // a warp's sums of a tile as the lanes have them
+    uint4 zeros[16];                         // what a token that did not choose an expert has there
     float weight[MAX_T * MAX_K];             // by (token, choice)
     int chosen[MAX_T * MAX_K];
     unsigned users[MAX_E];                   // tokens that chose an expert
@@ -249,61 +296,95 @@ struct alignas(16) Shared {
     unsigned mask[MAX_T * MAX_K];            // their tokens
     int first[MAX_T * MAX_K];                // where their tokens' weights begin in
     float factor[MAX_T * MAX_K];             // [slot][its tokens in order]
-    int2 unit[WARPS][NT];                    // [team][tile]: (slot, first column) of a team's units
+    int2 count[MAX_E / 32];                  // of 32 experts: chosen ones, and their tokens together
+    int2 unit[WARPS][NT];                    // [team][tile]: (slot, unit) of a team's units
     int active;
     int go;
 };
 static_assert(sizeof(Shared) % 16 == 0, "rows of 16-byte pieces lie behind it");
 
-// Warp t: token t's choices, as the router kernels choose (the lowest index among equals).  A NaN among a token's logits makes its weights NaN.
-__device__ __forceinline__ void choose(const Params& p, Shared& sm, float* score, int t) {
+// A float as a number in its order; NaN lowest
+__device__ __forceinline__ uint32_t order(float v) {
+    const uint32_t b = __float_as_uint(v);
+    return v == v ? (b & 0x80000000u ? ~b : b | 0x80000000u) : 0u;
+}
+
+// Token t's choices by a warp, as the router kernels choose (the lowest index among equals).  A NaN among a token's logits makes
+// its weights NaN.  (Code that runs once waits for its instructions: it is short, and its loops are loops.)
+__device__ __forceinline__ void choose(const Params& p, Shared& sm, uint32_t* rest, int t) {
     const int lane = threadIdx.x & 31;
-    float* c_s = score + (size_t)t * 2 * p.E;             // what the choice goes by, then what the weights go by
-    float* s_s = c_s + p.E;
     const float* z = p.z + (size_t)t * p.E;
-    bool broken = false;
-    for (int e = lane; e < p.E; e += 32) {
+    auto score = [&](int e) {
         const float v = z[e] + (p.bias ? p.bias[e] : 0.0f);
-        const float s = p.softmax ? v : 1.0f / (1.0f + expf(-v));
-        broken |= s != s;
-        s_s[e] = s;
-        c_s[e] = p.correction ? s + p.correction[e] : s;
+        return p.softmax ? v : 1.0f / (1.0f + expf(-v));
+    };
+    bool broken = false;
+    int mine = 0;                                          // lane j keeps the j-th choice
+    // The largest of all lanes' `best`, and the lowest of the experts that have it; nothing but NaN left: any, but a valid one
+    auto pick = [&](int j, uint32_t best, int at) {
+        const uint32_t top = __reduce_max_sync(0xffffffffu, best);
+        at = (int)__reduce_min_sync(0xffffffffu, best == top && best ? (unsigned)at : (unsigned)p.E);
+        if (at >= p.E) at = j;
+        if (lane == j) mine = at;
+        return at;
+    };
+    if (p.E <= 128) {                                      // four a lane, in registers
+        uint32_t key[4];
+        float s[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[i] = lane + 32 * i < p.E ? score(lane + 32 * i) : 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            broken |= s[i] != s[i];
+            key[i] = lane + 32 * i < p.E ? order(p.correction ? s[i] + p.correction[lane + 32 * i] : s[i]) : 0u;
+        }
+#pragma unroll 1
+        for (int j = 0; j < p.k; ++j) {
+            uint32_t best = key[0];
+            int at = lane;
+#pragma unroll
+            for (int i = 1; i < 4; ++i)
+                if (key[i] > best) { best = key[i]; at = lane + 32 * i; }      // the first of equals
+            at = pick(j, best, at);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (at == lane + 32 * i) key[i] = 0u;
+        }
+    } else {
+#pragma unroll 4
+        for (int e = lane; e < p.E; e += 32) {
+            const float s = score(e);
+            broken |= s != s;
+            rest[e] = order(p.correction ? s + p.correction[e] : s);
+        }
+#pragma unroll 1
+        for (int j = 0; j < p.k; ++j) {
+            uint32_t best = 0;
+            int at = p.E;
+#pragma unroll 4
+            for (int e = lane; e < p.E; e += 32)
+                if (rest[e] > best) { best = rest[e]; at = e; }
+            at = pick(j, best, at);
+            if (at % 32 == lane) rest[at] = 0u;
+        }
     }
     broken = __any_sync(0xffffffffu, broken);
-    __syncwarp();
-    float total = 0.0f, top = 0.0f, mine = 0.0f;
-    for (int j = 0; j < p.k; ++j) {
-        float best = -INFINITY;
-        int at = 0x7fffffff;
-        for (int e = lane; e < p.E; e += 32) {
-            const float c = c_s[e];
-            if (c > best) { best = c; at = e; }
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            const float ob = __shfl_xor_sync(0xffffffffu, best, o);
-            const int oa = __shfl_xor_sync(0xffffffffu, at, o);
-            if (ob > best || (ob == best && oa < at)) { best = ob; at = oa; }
-        }
-        if (at >= p.E) at = j < p.E ? j : 0;               // no score is above minus infinity: any expert, but a valid one
-        float s = s_s[at];
-        if (p.softmax) {
-            if (j == 0) top = s;
-            s = expf(s - top);
-        }
-        total += s;
-        if (lane == j) mine = s;
-        if (lane == 0) {
-            sm.chosen[t * p.k + j] = at;
-            c_s[at] = -INFINITY;
-        }
-        __syncwarp();
-    }
+    float s = 0.0f;
     if (lane < p.k) {
-        float w = p.softmax ? mine * (p.scale / total) : mine * (p.renormalize ? p.scale / total : p.scale);
-        sm.weight[t * p.k + lane] = broken ? __int_as_float(0x7fc00000) : w;
+        s = score(mine);
+        atomicOr(&sm.users[mine], 1u << t);
+        sm.chosen[t * p.k + lane] = mine;
     }
+    if (p.softmax) {                                       // the first choice has the largest logit
+        const float top = __shfl_sync(0xffffffffu, s, 0);
+        s = lane < p.k ? expf(s - top) : 0.0f;
+    }
+    const float total = warp_sum(s);
+    if (lane < p.k) sm.weight[t * p.k + lane] = broken ? __int_as_float(0x7fc00000) : s * (p.softmax || p.renormalize ? p.scale / total : p.scale);
 }
+
+// Bytes of shared memory for the choice
+__host__ __device__ __forceinline__ size_t scores_bytes(int T, int E) { return ((size_t)T * E * 4 + 15) / 16 * 16; }
 
 // A barrier of `threads` threads of the CTA, a multiple of 32
 __device__ __forceinline__ void named_barrier(int id, int threads) {
@@ -329,56 +410,64 @@ __device__ __forceinline__ bool grid_barrier(int* counter, int* go) {
     return *go != 0;
 }
 
-template <bool W8, bool WIDE>
+template <bool W8, int COLS>
 __global__ void __launch_bounds__(THREADS, 1)
 moe_few_kernel(const Params p) {
     extern __shared__ __align__(16) uint8_t smem[];
     Shared& sm = *reinterpret_cast<Shared*>(smem);
-    float* score = reinterpret_cast<float*>(smem + sizeof(Shared));      // [T, 2, E]
+    uint32_t* const rest = reinterpret_cast<uint32_t*>(smem + sizeof(Shared));      // [T, E]
     constexpr int SIZE = W8 ? 1 : 2;                                      // bytes of a weight
+    constexpr int X_STEP = W8 ? 2 * STEP : STEP;                          // bytes of a step of a token's row
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
     // rows x in shared memory: a pitch of 64 bytes over a multiple of 128 puts two rows' 64 bytes into different banks
     const int pitch = (p.ldx + 127) / 128 * 128 + 64;
-    uint8_t* const staged = smem + sizeof(Shared) + ((size_t)p.T * 2 * p.E * 4 + 15) / 16 * 16;
+    uint8_t* const staged = smem + sizeof(Shared) + scores_bytes(p.T, p.E);
+    for (int e = threadIdx.x; e < p.E; e += THREADS) sm.users[e] = 0;
+    if (threadIdx.x < 16) sm.zeros[threadIdx.x] = make_uint4(0u, 0u, 0u, 0u);
+    __syncthreads();
     pdl_wait();
     if (p.staged) {
         const int each = p.ldx / 16;
-        for (int i = threadIdx.x; i < p.T * each; i += THREADS) {
-            const int r = i / each, c = (i - r * each) * 16;
-            mma16::cp_async_16(staged + (size_t)r * pitch + c, p.x + (size_t)r * p.ldx + c, 16);
-        }
+#pragma unroll 1
+        for (int r = warp; r < p.T; r += WARPS)
+#pragma unroll 4
+            for (int c = lane; c < each; c += 32) mma16::cp_async_16(staged + (size_t)r * pitch + c * 16, p.x + (size_t)r * p.ldx + c * 16, 16);
     }
     mma16::cp_async_commit();
 
     // ---- who goes where (every CTA for itself) ------------------------------------------------
-    for (int e = threadIdx.x; e < p.E; e += THREADS) sm.users[e] = 0;
-    for (int t = warp; t < p.T; t += WARPS) choose(p, sm, score, t);
+    if (warp < p.T) choose(p, sm, rest + warp * p.E, warp);
     __syncthreads();
-    for (int i = threadIdx.x; i < p.T * p.k; i += THREADS) atomicOr(&sm.users[sm.chosen[i]], 1u << (i / p.k));
+    // the chosen experts in ascending order: a warp counts 32 experts, and those in front of them
+    const int chunks = (p.E + 31) / 32;
+#pragma unroll 1
+    for (int i = warp; i < chunks; i += WARPS) {
+        const int e = i * 32 + lane;
+        const unsigned users = e < p.E ? sm.users[e] : 0u;
+        const unsigned any = __ballot_sync(0xffffffffu, users != 0), pairs = __reduce_add_sync(0xffffffffu, __popc(users));
+        if (lane == 0) sm.count[i] = make_int2(__popc(any), (int)pairs);
+    }
     __syncthreads();
-    if (warp == 0) {
-        int n = 0, before = 0;
-        for (int e0 = 0; e0 < p.E; e0 += 32) {
-            const int e = e0 + lane;
-            const unsigned m = e < p.E ? sm.users[e] : 0u;
-            const unsigned any = __ballot_sync(0xffffffffu, m != 0);
-            int incl = __popc(m);
+#pragma unroll 1
+    for (int i = warp; i < chunks; i += WARPS) {
+        const int e = i * 32 + lane;
+        const unsigned users = e < p.E ? sm.users[e] : 0u, any = __ballot_sync(0xffffffffu, users != 0);
+        const int2 here = lane < i ? sm.count[lane] : make_int2(0, 0);
+        const int n = (int)__reduce_add_sync(0xffffffffu, (unsigned)here.x), before = (int)__reduce_add_sync(0xffffffffu, (unsigned)here.y);
+        int incl = __popc(users);
 #pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int v = __shfl_up_sync(0xffffffffu, incl, o);
-                if (lane >= o) incl += v;
-            }
-            if (m) {
-                const int s = n + __popc(any & ((1u << lane) - 1));
-                sm.slot[e] = s;
-                sm.expert[s] = e;
-                sm.mask[s] = m;
-                sm.first[s] = before + incl - __popc(m);
-            }
-            n += __popc(any);
-            before += __shfl_sync(0xffffffffu, incl, 31);
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += v;
         }
-        if (lane == 0) sm.active = n;
+        if (users) {
+            const int s = n + __popc(any & ((1u << lane) - 1));
+            sm.slot[e] = s;
+            sm.expert[s] = e;
+            sm.mask[s] = users;
+            sm.first[s] = before + incl - __popc(users);
+        }
+        if (lane == 0 && i + 1 == chunks) sm.active = n + __popc(any);
     }
     __syncthreads();
     for (int i = threadIdx.x; i < p.T * p.k; i += THREADS) {
@@ -389,142 +478,213 @@ moe_few_kernel(const Params p) {
     __syncthreads();
     const int active = sm.active;
 
-    uint4 w[NT][2];                                                       // the step that is on its way
-    float acc[NT][4];
+    uint4 w[NT][2][2];                                                    // the step that is on its way
+    float acc[NT][COLS][4];
     auto clear = [&]() {
 #pragma unroll
         for (int i = 0; i < NT; ++i)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) acc[i][j] = 0.0f;
+            for (int n = 0; n < COLS; ++n)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[i][n][j] = 0.0f;
     };
     auto leave = [&]() {                                                  // this warp's sums for the others to add
 #pragma unroll
-        for (int i = 0; i < NT; ++i) {
-            float (&d)[2][MAX_T][4] = sm.part[warp][i];
-            *reinterpret_cast<float2*>(&d[t4 >> 1][g][2 * (t4 & 1)]) = make_float2(acc[i][0], acc[i][1]);
-            if (WIDE) *reinterpret_cast<float2*>(&d[t4 >> 1][g + 8][2 * (t4 & 1)]) = make_float2(acc[i][2], acc[i][3]);
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+            for (int n = 0; n < COLS; ++n) sm.part[warp][i][n][lane] = make_float4(acc[i][n][0], acc[i][n][1], acc[i][n][2], acc[i][n][3]);
+    };
+    auto joined = [&](int from, int warps, int i, int n, int l) {         // the warps' sums together
+        float4 v = sm.part[from][i][n][l];
+        for (int q = 1; q < warps; ++q) {
+            const float4 o = sm.part[from + q][i][n][l];
+            v.x += o.x;
+            v.y += o.y;
+            v.z += o.z;
+            v.w += o.w;
         }
+        return v;
     };
 
-    // ---- act: units of four gate rows and their up rows, dealt out over the teams, up to NT units at a time -------------
+    // ---- act: units of eight gate rows and their up rows, dealt out over the teams, up to NT units at a time ------------
     {
         const int team = p.team, me = warp % team, my_team = warp / team, teams = gridDim.x * (WARPS / team);
-        const int per = (p.I + 3) / 4, NB = (2 * p.I + fp8::BLOCK - 1) / fp8::BLOCK, KB = (p.H + fp8::BLOCK - 1) / fp8::BLOCK;
+        const int per = (p.I + 7) / 8, NB = (2 * p.I + fp8::BLOCK - 1) / fp8::BLOCK, KB = (p.H + fp8::BLOCK - 1) / fp8::BLOCK;
         const long long units = (long long)active * per;
         const int index = blockIdx.x * (WARPS / team) + my_team;
-        const int u_begin = (int)(units * index / teams), u_count = (int)(units * (index + 1) / teams) - u_begin;
-        const int groups = (u_count + NT - 1) / NT, size = groups ? u_count / groups : 0, larger = groups ? u_count - size * groups : 0;
+        const int u_begin = (int)(units * index / teams), u_end = (int)(units * (index + 1) / teams);
         const int len = p.H * SIZE, steps = (len + STEP - 1) / STEP;
         const uint8_t* const x = p.staged ? staged : p.x;
         const unsigned ld = p.staged ? pitch : p.ldx;
-        const uint8_t* const x_lo = g < p.T ? x + g * ld : nullptr;
-        const uint8_t* const x_hi = WIDE && g + 8 < p.T ? x + (g + 8) * ld : nullptr;
-        int a = u_begin / per, c = u_begin - a * per;                     // slot and unit within of the next group's first
-        const uint8_t* row[NT];
-        unsigned scale_at[NT];
-        int next_tiles = 0;
-        unsigned next_scale_at[NT];
-        int2 next_unit = make_int2(0, 0);                                 // lane i < NT: of unit i
-        // the rows and scales of group i, whose first unit is (a, c); on to the group behind it
-        auto look_up = [&](int i) {
-            next_tiles = size + (i < larger);
+        const uint8_t* x_row[COLS];                                       // (a token there is not has another's row: it is dropped)
+        const float* x_scale[COLS];
+#pragma unroll
+        for (int n = 0; n < COLS; ++n) {
+            x_row[n] = x + min(8 * n + g, p.T - 1) * ld;
+            x_scale[n] = p.x_scale + min(8 * n + 2 * t4, p.T - 1) * KB;
+        }
+        const int odd[2] = {2 * t4 + 1 < p.T ? KB : 0, 8 + 2 * t4 + 1 < p.T ? KB : 0};
+        const size_t to_up = (size_t)p.I * p.ldg;
+        // the units of a group: slot, column, this lane's gate row (the up row lies to_up bytes on) and both rows' scales
+        struct Unit {
+            const uint8_t* gate;
+            int slot, unit;
+            unsigned scale[2];
+        } next[NT];
+        int a = u_begin / per, c = u_begin - a * per, next_tiles = 0;     // of the first unit behind the groups looked up
+        auto look_up = [&](int u) {
+            next_tiles = min(NT, u_end - u);
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
-                const int e = sm.expert[a], r = min(c * 4 + (g & 3), p.I - 1);
-                row[j] = static_cast<const uint8_t*>(p.gate_up) + (unsigned long long)(unsigned)(e * 2 * p.I + (g < 4 ? r : p.I + r)) * (unsigned)p.ldg;
+                const int e = sm.expert[a], r = min(c * 8 + g, p.I - 1);
+                next[j].slot = a;
+                next[j].unit = c;
+                next[j].gate = static_cast<const uint8_t*>(p.gate_up) + (unsigned long long)(unsigned)(e * 2 * p.I + r) * (unsigned)p.ldg;
                 if constexpr (W8) {
-                    // sums 2 t4 and 2 t4 + 1 of the tile: gate rows for t4 < 2, up rows above; as I is even two neighbours lie
-                    // in one block of 128 rows
-                    const int n = min(c * 4 + 2 * (t4 & 1), p.I - 2) + (t4 < 2 ? 0 : p.I);
-                    next_scale_at[j] = (unsigned)(e * NB + n / fp8::BLOCK) * (unsigned)KB;
+                    next[j].scale[0] = (unsigned)(e * NB + r / fp8::BLOCK) * (unsigned)KB;
+                    next[j].scale[1] = (unsigned)(e * NB + (p.I + r) / fp8::BLOCK) * (unsigned)KB;
                 }
-                if (lane == j) next_unit = make_int2(a, c * 4);
-                if (j + 1 <= next_tiles && !(j + 1 == next_tiles && i + 1 == groups) && ++c == per) {
+                if (u + j + 1 < u_end && j < next_tiles && ++c == per) {
                     c = 0;
                     ++a;
                 }
             }
         };
-        if (groups) {
-            look_up(0);
-            fetch(w, row, next_tiles, me * STEP, len);                    // (a team has at most a quarter as many warps as steps)
+        auto fetch_at = [&](int at) {
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+                if (j < next_tiles) fetch(w[j], next[j].gate, next[j].gate + to_up, at, len);
+        };
+        // two lanes of the team's first warp ask for the rows of a unit of the group looked up last
+        auto ask = [&]() {
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+                const int r = next[j].unit * 8, rows = min(8, p.I - r);
+                if (me == 0 && lane < 2 && j < next_tiles)                // (lanes 0 and 1 have the unit's first row)
+                    ask_for(next[j].gate + lane * to_up, (unsigned)(rows - 1) * (unsigned)p.ldg + (unsigned)(len + 15) / 16 * 16);
+            }
+        };
+        if (u_begin < u_end) {
+            look_up(u_begin);
+            ask();
+            fetch_at(me * STEP);                                          // (a team has at most a quarter as many warps as steps)
         }
-        for (int i = 0; i < groups; ++i) {
+        for (int u = u_begin; u < u_end; u += NT) {
             clear();
             const int tiles = next_tiles;
-            const int2 unit = next_unit;
+            Unit now[NT];
 #pragma unroll
-            for (int j = 0; j < NT; ++j) scale_at[j] = next_scale_at[j];
+            for (int j = 0; j < NT; ++j) now[j] = next[j];
             for (int s = me; s < steps; s += team) {
-                const int at = s * STEP, x_at = s * (W8 ? 2 * STEP : STEP);
-                float scale[NT], f_lo = 0.0f, f_hi = 0.0f;
+                Tokens<W8> xs[COLS];
+                Factors<COLS> f[NT];
+#pragma unroll
+                for (int n = 0; n < COLS; ++n) xs[n].load(x_row[n] + s * X_STEP, p.ldx - s * X_STEP);
                 if constexpr (W8) {
 #pragma unroll
-                    for (int j = 0; j < NT; ++j) scale[j] = p.gate_up_scale[scale_at[j] + s];
-                    if (g < p.T) f_lo = p.x_scale[g * KB + s];
-                    if (WIDE && g + 8 < p.T) f_hi = p.x_scale[(g + 8) * KB + s];
+                    for (int j = 0; j < NT; ++j) {
+                        f[j].row[0] = p.gate_up_scale[now[j].scale[0] + s];
+                        f[j].row[1] = p.gate_up_scale[now[j].scale[1] + s];
+#pragma unroll
+                        for (int n = 0; n < COLS; ++n) {
+                            f[j].token[n][0] = x_scale[n][s];
+                            f[j].token[n][1] = x_scale[n][s + odd[n]];
+                        }
+                    }
                 }
-                multiply<W8, WIDE>(acc, w, tiles, x_lo ? x_lo + x_at : nullptr, WIDE && x_hi ? x_hi + x_at : nullptr, p.ldx - x_at, f_lo, f_hi, scale);
+#pragma unroll
+                for (int j = 0; j < NT; ++j)
+                    if (j < tiles) accumulate<W8, COLS>(acc[j], w[j], xs, f[j]);
                 if (s + team < steps) {
-                    fetch(w, row, tiles, at + team * STEP, len);
-                } else if (i + 1 < groups) {
-                    look_up(i + 1);
-                    fetch(w, row, next_tiles, me * STEP, len);
+                    fetch_at((s + team) * STEP);
+                } else if (u + NT < u_end) {
+                    look_up(u + NT);
+                    fetch_at(me * STEP);
+                    ask();
                 }
             }
             named_barrier(1 + my_team, team * 32);                        // the sums before these are added by now
-            if (me == 0 && lane < NT) sm.unit[my_team][lane] = lane < tiles ? unit : make_int2(-1, 0);
+            if (me == 0 && lane == 0) {
+#pragma unroll
+                for (int j = 0; j < NT; ++j) sm.unit[my_team][j] = j < tiles ? make_int2(now[j].slot, now[j].unit) : make_int2(-1, 0);
+            }
             leave();
             named_barrier(1 + my_team, team * 32);
-            for (int o = me * 32 + lane; o < NT * MAX_T * 4; o += team * 32) {
-                const int j = o / (MAX_T * 4), t = o / 4 % MAX_T;
+            for (int o = me * 32 + lane; o < NT * COLS * 32; o += team * 32) {
+                const int j = o / (COLS * 32), n = o / 32 % COLS, l = o % 32;
                 const int2 unit = sm.unit[my_team][j];
-                const int col = unit.y + o % 4;
-                if (unit.x < 0 || t >= p.T || col >= p.I) continue;
+                const int col = unit.y * 8 + l / 4;
+                if (unit.x < 0 || col >= p.I) continue;
+                const float4 v = joined(my_team * team, team, j, n, l);
                 const unsigned m = sm.mask[unit.x];
-                if (!(m >> t & 1)) continue;
-                float gv = 0.0f, uv = 0.0f;
-                for (int q = 0; q < team; ++q) {
-                    gv += sm.part[my_team * team + q][j][0][t][o % 4];
-                    uv += sm.part[my_team * team + q][j][1][t][o % 4];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int t = 8 * n + 2 * (l % 4) + i;
+                    if (!(m >> t & 1)) continue;
+                    float gv = i ? v.y : v.x, uv = i ? v.w : v.z;
+                    const float weight = sm.factor[sm.first[unit.x] + __popc(m & ((1u << t) - 1))];
+                    if (p.on_input) { gv *= weight; uv *= weight; }
+                    float h = gv / (1.0f + expf(-gv)) * uv;
+                    if (!p.on_input) h *= weight;
+                    const size_t at = ((size_t)unit.x * p.T + t) * p.Ip + col;
+                    if constexpr (W8) static_cast<float*>(p.act)[at] = h;
+                    else static_cast<bf16*>(p.act)[at] = __float2bfloat16_rn(h);
                 }
-                const float f = sm.factor[sm.first[unit.x] + __popc(m & ((1u << t) - 1))];
-                if (p.on_input) { gv *= f; uv *= f; }
-                float v = gv / (1.0f + expf(-gv)) * uv;
-                if (!p.on_input) v *= f;
-                const size_t at = ((size_t)unit.x * p.T + t) * p.Ip + col;
-                if constexpr (W8) static_cast<float*>(p.act)[at] = v;
-                else static_cast<bf16*>(p.act)[at] = __float2bfloat16_rn(v);
             }
         }
     }
 
-    // ---- y: rows of the down matrices, dealt out over the grid; the sum runs over all chosen experts.  The first weights
-    // are asked for ahead of the barrier. ---------------------------------------------------------------------------------
-    const int pairs = (p.H + 1) / 2, NB = (p.H + fp8::BLOCK - 1) / fp8::BLOCK, KB = (p.I + fp8::BLOCK - 1) / fp8::BLOCK;
-    const int r_begin = 2 * (int)((long long)pairs * blockIdx.x / gridDim.x);
-    const int r_end = min(p.H, 2 * (int)((long long)pairs * (blockIdx.x + 1) / gridDim.x));
-    const int all_tiles = (r_end - r_begin + 7) / 8, groups = (all_tiles + NT - 1) / NT;
-    const int len = p.I * SIZE, per = (len + STEP - 1) / STEP, steps = active * per;
-    // steps go round the warps: (slot, step within) and on by WARPS
-    const int round_a = WARPS / per, round_s = WARPS - round_a * per, warp_a = warp / per, warp_s = warp - warp_a * per;
-    int a = warp_a, k = warp_s;                                           // of the step on its way
-    unsigned row_at[NT];
-    auto rows_of = [&](int first) {
-#pragma unroll
-        for (int i = 0; i < NT; ++i) row_at[i] = (unsigned)min(r_begin + (first + i) * 8 + g, r_end - 1);
+    // ---- y: rows of the down matrices, dealt out over the grid, sixteen or thirty-two at a time; the sum runs over the blocks
+    // of K of all chosen experts.  The first weights are asked for ahead of the barrier. -----------------------------------
+    const int NB = (p.H + fp8::BLOCK - 1) / fp8::BLOCK, KB = (p.I + fp8::BLOCK - 1) / fp8::BLOCK;
+    const int r_begin = (int)((long long)p.H * blockIdx.x / gridDim.x), r_end = (int)((long long)p.H * (blockIdx.x + 1) / gridDim.x);
+    const int len = p.I * SIZE, per = (len + STEP - 1) / STEP, items = active * per;
+    // the rows of this CTA of the expert in a slot; the warp that begins an expert asks for the one behind the next
+    auto ask = [&](int slot) {
+        if (lane == 0 && slot < active && r_end > r_begin)
+            ask_for(static_cast<const uint8_t*>(p.down) + ((size_t)sm.expert[slot] * p.H + r_begin) * p.ldd,
+                    (unsigned)(r_end - r_begin - 1) * (unsigned)p.ldd + (unsigned)(len + 15) / 16 * 16);
     };
-    auto fetch_down = [&](int tiles) {
-        const uint8_t* const base = static_cast<const uint8_t*>(p.down) + (size_t)sm.expert[a] * p.H * p.ldd;
-        const uint8_t* row[NT];
-#pragma unroll
-        for (int i = 0; i < NT; ++i) row[i] = base + (unsigned long long)row_at[i] * (unsigned)p.ldd;
-        fetch(w, row, tiles, k * STEP, len);
+    // A step of a warp is two tiles of one block, or one tile of two blocks where that is all there is: a block in a row of
+    // K is an item (slot, block), and the items go round the warps
+    struct Item {
+        int slot, block;
     };
-    auto tile_of = [&](int i) { return all_tiles * i / groups; };         // group i: tiles from ... on
-    if (groups && warp < steps) {
-        rows_of(0);
-        fetch_down(tile_of(1));
+    int r0 = r_begin;                                                     // first row of the group on its way
+    bool two = false;                                                     // whether it has two tiles
+    Item item[2];                                                         // what is on its way (two tiles: one)
+    int at = 0;                                                           // items of this warp before it
+    auto item_of = [&](int i) {
+        Item r;
+        r.slot = i / per;
+        r.block = i - r.slot * per;
+        return r;
+    };
+    auto down_row = [&](int slot, int r) {
+        return static_cast<const uint8_t*>(p.down) + ((size_t)sm.expert[slot] * p.H + min(r, r_end - 1)) * p.ldd;
+    };
+    auto fetch_items = [&]() {                                            // from `at` on
+        if (two) {
+            const int i = at * WARPS + warp;
+            if (i >= items) return;
+            item[0] = item_of(i);
+            fetch(w[0], down_row(item[0].slot, r0 + g), down_row(item[0].slot, r0 + 8 + g), item[0].block * STEP, len);
+            fetch(w[1], down_row(item[0].slot, r0 + 16 + g), down_row(item[0].slot, r0 + 24 + g), item[0].block * STEP, len);
+        } else {
+#pragma unroll
+            for (int f = 0; f < 2; ++f) {
+                const int i = (at + f) * WARPS + warp;
+                item[f].slot = -1;
+                if (i >= items) continue;
+                item[f] = item_of(i);
+                fetch(w[f], down_row(item[f].slot, r0 + g), down_row(item[f].slot, r0 + 8 + g), item[f].block * STEP, len);
+            }
+        }
+    };
+    if (warp < 2) ask(warp);
+    if (r_begin < r_end) {
+        two = r_end - r0 > 16;
+        fetch_items();
     }
     bool met = grid_barrier(p.barrier, &sm.go);
     if constexpr (W8) {
@@ -553,66 +713,97 @@ moe_few_kernel(const Params p) {
         if (threadIdx.x == 0) atomicExch(p.status, 19);
         return;
     }
-    for (int i = 0; i < groups; ++i) {
-        const int first = tile_of(i), tiles = tile_of(i + 1) - first, r0 = r_begin + first * 8, r1 = min(r_end, r0 + tiles * 8);
-        unsigned block[NT];                                               // (rows from an even one on: both sums' lie in one block)
+    const uint8_t* const act = W8 ? reinterpret_cast<const uint8_t*>(p.act16) : static_cast<const uint8_t*>(p.act);
+    // the tokens' elements of an item, and what its products are multiplied by in the rows from r on
+    auto tokens_of = [&](Tokens<W8> (&xs)[COLS], const Item& i) {
+        const unsigned m = sm.mask[i.slot];
 #pragma unroll
-        for (int j = 0; j < NT; ++j) block[j] = (unsigned)min(r0 + j * 8 + 2 * t4, p.H - 1) / fp8::BLOCK;
-        clear();
-        for (int s = warp; s < steps; s += WARPS) {
-            const int e = sm.expert[a], from = k;
-            const unsigned m = sm.mask[a], r = (unsigned)(a * p.T + g);
-            const bool in_lo = m >> g & 1, in_hi = WIDE && (m >> (g + 8) & 1);
-            const uint8_t* lo = nullptr;
-            const uint8_t* hi = nullptr;
-            float scale[NT], f_lo = 0.0f, f_hi = 0.0f;
-            const uint8_t* const act = W8 ? reinterpret_cast<const uint8_t*>(p.act16) : static_cast<const uint8_t*>(p.act);
-            const unsigned x_at = from * (W8 ? 2 * STEP : STEP);
-            if (in_lo) lo = act + (size_t)r * 2 * p.Ip + x_at;
-            if (in_hi) hi = act + (size_t)(r + 8) * 2 * p.Ip + x_at;
-            if constexpr (W8) {
-                if (in_lo) f_lo = p.act_scale[r * KB + from];
-                if (in_hi) f_hi = p.act_scale[(r + 8) * KB + from];
-#pragma unroll
-                for (int j = 0; j < NT; ++j) scale[j] = p.down_scale[(unsigned)(e * NB + block[j]) * (unsigned)KB + from];
-            }
-            multiply<W8, WIDE>(acc, w, tiles, lo, hi, W8 ? 2 * STEP : len - from * STEP, f_lo, f_hi, scale);
-            a += round_a;
-            k += round_s;
-            if (k >= per) {
-                k -= per;
-                ++a;
-            }
-            if (s + WARPS < steps) {
-                fetch_down(tiles);
-            } else if (i + 1 < groups) {
-                a = warp_a;
-                k = warp_s;
-                rows_of(first + tiles);
-                fetch_down(tile_of(i + 2) - first - tiles);
-            }
+        for (int n = 0; n < COLS; ++n) {
+            const int t = 8 * n + g;
+            const bool in = m >> t & 1;
+            xs[n].load(in ? act + ((size_t)i.slot * p.T + t) * 2 * p.Ip + i.block * X_STEP : reinterpret_cast<const uint8_t*>(sm.zeros),
+                       W8 ? X_STEP : in ? len - i.block * X_STEP : X_STEP);
         }
-        if (i > 0) __syncthreads();                                       // the sums before these are added by now
+    };
+    auto factors_of = [&](Factors<COLS>& f, const Item& i, int r) {
+        if constexpr (W8) {
+            const unsigned m = sm.mask[i.slot], e = sm.expert[i.slot] * NB;
+            f.row[0] = p.down_scale[(e + (unsigned)min(r + g, p.H - 1) / fp8::BLOCK) * (unsigned)KB + i.block];
+            f.row[1] = p.down_scale[(e + (unsigned)min(r + 8 + g, p.H - 1) / fp8::BLOCK) * (unsigned)KB + i.block];
+#pragma unroll
+            for (int n = 0; n < COLS; ++n)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const int t = 8 * n + 2 * t4 + j;
+                    f.token[n][j] = m >> t & 1 ? p.act_scale[(unsigned)(i.slot * p.T + t) * (unsigned)KB + i.block] : 0.0f;
+                }
+        }
+    };
+    for (int r = r_begin, rows; r < r_end; r += rows) {
+        const bool pair = two;
+        rows = pair ? 32 : 16;
+        clear();
+        for (at = 0; at * WARPS + warp < items;) {
+            Tokens<W8> xs[COLS];
+            Factors<COLS> f;
+            const Item first = item[0], second = item[1];
+            tokens_of(xs, first);
+            factors_of(f, first, r);
+            if (pair) {
+                if (r == r_begin && first.block == 0) ask(first.slot + 2);
+                accumulate<W8, COLS>(acc[0], w[0], xs, f);
+                if constexpr (W8) {
+                    f.row[0] = p.down_scale[((unsigned)sm.expert[first.slot] * NB + (unsigned)min(r + 16 + g, p.H - 1) / fp8::BLOCK) * (unsigned)KB + first.block];
+                    f.row[1] = p.down_scale[((unsigned)sm.expert[first.slot] * NB + (unsigned)min(r + 24 + g, p.H - 1) / fp8::BLOCK) * (unsigned)KB + first.block];
+                }
+                accumulate<W8, COLS>(acc[1], w[1], xs, f);
+                ++at;
+            } else {
+                if (r == r_begin && first.block == 0) ask(first.slot + 2);
+                accumulate<W8, COLS>(acc[0], w[0], xs, f);
+                if (second.slot >= 0) {
+                    if (r == r_begin && second.block == 0) ask(second.slot + 2);
+                    tokens_of(xs, second);
+                    factors_of(f, second, r);
+                    accumulate<W8, COLS>(acc[0], w[1], xs, f);
+                }
+                at += 2;
+            }
+            if (at * WARPS + warp < items) fetch_items();
+        }
+        // the next group's first weights are on their way while these sums are joined
+        if (r + rows < r_end) {
+            r0 = r + rows;
+            two = r_end - r0 > 16;
+            at = 0;
+            fetch_items();
+        }
+        if (r > r_begin) __syncthreads();                                 // the sums before these are added by now
         leave();
         __syncthreads();
-        for (int o = threadIdx.x; o < NT * 2 * MAX_T * 4; o += THREADS) {
-            const int j = o >> 7, half = o >> 6 & 1, t = o / 4 % MAX_T, c = o % 4, r = r0 + j * 8 + half * 4 + c;
-            if (r >= r1 || t >= p.T) continue;
-            float v = 0.0f;
+        if (threadIdx.x < NT * COLS * 32) {
+            const int j = threadIdx.x / (COLS * 32), n = threadIdx.x / 32 % COLS, l = threadIdx.x % 32;
+            if (j == 0 || pair) {
+                const float4 v = joined(0, WARPS, j, n, l);
+                const float x[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-            for (int q = 0; q < WARPS; ++q) v += sm.part[q][j][half][t][c];
-            const size_t to = (size_t)t * p.H + r;
-            if (p.add) v += p.add[to];
-            if (p.out_bf16) static_cast<bf16*>(p.out)[to] = __float2bfloat16_rn(v);
-            else static_cast<float*>(p.out)[to] = v;
+                for (int i = 0; i < 4; ++i) {
+                    const int row = r + 16 * j + l / 4 + 8 * (i / 2), t = 8 * n + 2 * (l % 4) + i % 2;
+                    if (row >= r_end || t >= p.T) continue;
+                    const size_t to = (size_t)t * p.H + row;
+                    const float y = p.add ? x[i] + p.add[to] : x[i];
+                    if (p.out_bf16) static_cast<bf16*>(p.out)[to] = __float2bfloat16_rn(y);
+                    else static_cast<float*>(p.out)[to] = y;
+                }
+            }
         }
     }
 }
 
-template <bool W8, bool WIDE>
+template <bool W8, int COLS>
 int launch(Params& p, int sms, cudaStream_t stream) {
-    const auto kernel = moe_few_kernel<W8, WIDE>;
-    const size_t scores = ((size_t)p.T * 2 * p.E * sizeof(float) + 15) / 16 * 16;
+    const auto kernel = moe_few_kernel<W8, COLS>;
+    const size_t scores = scores_bytes(p.T, p.E);
     const size_t rows = (size_t)p.T * ((p.ldx + 127) / 128 * 128 + 64);
     constexpr size_t MOST = 226 * 1024;
     p.staged = sizeof(Shared) + scores + rows <= MOST;
@@ -693,6 +884,6 @@ SHARPI_API int sharpi_moe_few(const void* x, int x_dtype, int ldx, const void* h
     p.team = 1;
     while (p.team < WARPS && p.team * 8 <= steps) p.team *= 2;
     const bool wide = T > 8;
-    return w8 ? (wide ? launch<true, true>(p, sms, stream) : launch<true, false>(p, sms, stream))
-              : (wide ? launch<false, true>(p, sms, stream) : launch<false, false>(p, sms, stream));
+    return w8 ? (wide ? launch<true, 2>(p, sms, stream) : launch<true, 1>(p, sms, stream))
+              : (wide ? launch<false, 2>(p, sms, stream) : launch<false, 1>(p, sms, stream));
 }
