@@ -8,7 +8,7 @@
 // CTA an SM, weight rows dealt out evenly over the warps whatever expert they belong to, each weight read once, in 16-byte
 // pieces straight into registers.  Teams of 1 to 16 warps share K in turn (the more K has, the more); a warp asks for its next
 // step of 4 KB when it has multiplied the last (up to 64 KB an SM in flight; reading at 6.4 TB/s with a microsecond of latency
-// takes 44 KB), and rows are asked into L2 before that.  Weights are the 16-row operand of the MMA (eight gate rows and their up
+// takes 44 KB; asking whole rows into L2 ahead of that took 3 to 8 % longer).  Weights are the 16-row operand of the MMA (eight gate rows and their up
 // rows, or sixteen rows of the down matrix), tokens the eight columns; a column of a token that did not choose the expert is
 // computed and dropped (gate|up) or zero (down).  Because the down product is linear, a token's experts are one long sum over
 // (expert, inner element): act is multiplied by the router's weight before (weights on the output).  The warps' parts are added
@@ -72,12 +72,6 @@ __device__ __forceinline__ uint2 halves(const float (&v)[4], float s) {
     return make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
 }
 
-// Memory into L2, ahead of the loads: rows whose reads would wait for a step each then wait for L2 alone.  (Nothing is read by
-// it, so it may run ahead of whoever writes there.)
-__device__ __forceinline__ void ask_for(const void* p, unsigned bytes) {
-    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"(bytes) : "memory");
-}
-
 // One warp a (token, expert), the additions in the order of the router kernels for more tokens: lane l adds the elements
 // 128 i + 4 l + u in ascending i into chain u, the chains and then the lanes are added in a fixed order.
 template <typename T>
@@ -86,7 +80,6 @@ moe_few_router_kernel(const T* h, int ldh, const float* wr, int tokens, int H, i
                       const bf16* rows, int ld_rows, __half* rows16, int ld16, float* x_scale) {
     const int item = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
     const int e = item / tokens, t = item - e * tokens;
-    if (vec && t == 0 && e < E && lane == 0) ask_for(wr + (size_t)e * H, H * 4);
     pdl_wait();
     if (blockIdx.x == 0 && threadIdx.x < 2) barrier[threadIdx.x] = 0;
     if (e >= E) {                                        // e4m3 weights: the warps behind the experts' make h float16
@@ -508,12 +501,12 @@ moe_few_kernel(const Params p) {
 
     // ---- act: units of eight gate rows and their up rows, dealt out over the teams, up to NT units at a time ------------
     {
-        const int team = p.team, me = warp % team, my_team = warp / team, teams = gridDim.x * (WARPS / team);
         const int per = (p.I + 7) / 8, NB = (2 * p.I + fp8::BLOCK - 1) / fp8::BLOCK, KB = (p.H + fp8::BLOCK - 1) / fp8::BLOCK;
-        const long long units = (long long)active * per;
-        const int index = blockIdx.x * (WARPS / team) + my_team;
-        const int u_begin = (int)(units * index / teams), u_end = (int)(units * (index + 1) / teams);
         const int len = p.H * SIZE, steps = (len + STEP - 1) / STEP;
+        const long long units = (long long)active * per;
+        const int team = p.team;
+        const int me = warp % team, my_team = warp / team, teams = gridDim.x * (WARPS / team), index = blockIdx.x * (WARPS / team) + my_team;
+        const int u_begin = (int)(units * index / teams), u_end = (int)(units * (index + 1) / teams);
         const uint8_t* const x = p.staged ? staged : p.x;
         const unsigned ld = p.staged ? pitch : p.ldx;
         const uint8_t* x_row[COLS];                                       // (a token there is not has another's row: it is dropped)
@@ -555,18 +548,8 @@ moe_few_kernel(const Params p) {
             for (int j = 0; j < NT; ++j)
                 if (j < next_tiles) fetch(w[j], next[j].gate, next[j].gate + to_up, at, len);
         };
-        // two lanes of the team's first warp ask for the rows of a unit of the group looked up last
-        auto ask = [&]() {
-#pragma unroll
-            for (int j = 0; j < NT; ++j) {
-                const int r = next[j].unit * 8, rows = min(8, p.I - r);
-                if (me == 0 && lane < 2 && j < next_tiles)                // (lanes 0 and 1 have the unit's first row)
-                    ask_for(next[j].gate + lane * to_up, (unsigned)(rows - 1) * (unsigned)p.ldg + (unsigned)(len + 15) / 16 * 16);
-            }
-        };
         if (u_begin < u_end) {
             look_up(u_begin);
-            ask();
             fetch_at(me * STEP);                                          // (a team has at most a quarter as many warps as steps)
         }
         for (int u = u_begin; u < u_end; u += NT) {
@@ -600,7 +583,6 @@ moe_few_kernel(const Params p) {
                 } else if (u + NT < u_end) {
                     look_up(u + NT);
                     fetch_at(me * STEP);
-                    ask();
                 }
             }
             named_barrier(1 + my_team, team * 32);                        // the sums before these are added by now
@@ -639,12 +621,6 @@ moe_few_kernel(const Params p) {
     const int NB = (p.H + fp8::BLOCK - 1) / fp8::BLOCK, KB = (p.I + fp8::BLOCK - 1) / fp8::BLOCK;
     const int r_begin = (int)((long long)p.H * blockIdx.x / gridDim.x), r_end = (int)((long long)p.H * (blockIdx.x + 1) / gridDim.x);
     const int len = p.I * SIZE, per = (len + STEP - 1) / STEP, items = active * per;
-    // the rows of this CTA of the expert in a slot; the warp that begins an expert asks for the one behind the next
-    auto ask = [&](int slot) {
-        if (lane == 0 && slot < active && r_end > r_begin)
-            ask_for(static_cast<const uint8_t*>(p.down) + ((size_t)sm.expert[slot] * p.H + r_begin) * p.ldd,
-                    (unsigned)(r_end - r_begin - 1) * (unsigned)p.ldd + (unsigned)(len + 15) / 16 * 16);
-    };
     // A step of a warp is two tiles of one block, or one tile of two blocks where that is all there is: a block in a row of
     // K is an item (slot, block), and the items go round the warps
     struct Item {
@@ -681,7 +657,6 @@ moe_few_kernel(const Params p) {
             }
         }
     };
-    if (warp < 2) ask(warp);
     if (r_begin < r_end) {
         two = r_end - r0 > 16;
         fetch_items();
@@ -750,7 +725,6 @@ moe_few_kernel(const Params p) {
             tokens_of(xs, first);
             factors_of(f, first, r);
             if (pair) {
-                if (r == r_begin && first.block == 0) ask(first.slot + 2);
                 accumulate<W8, COLS>(acc[0], w[0], xs, f);
                 if constexpr (W8) {
                     f.row[0] = p.down_scale[((unsigned)sm.expert[first.slot] * NB + (unsigned)min(r + 16 + g, p.H - 1) / fp8::BLOCK) * (unsigned)KB + first.block];
@@ -759,10 +733,8 @@ moe_few_kernel(const Params p) {
                 accumulate<W8, COLS>(acc[1], w[1], xs, f);
                 ++at;
             } else {
-                if (r == r_begin && first.block == 0) ask(first.slot + 2);
                 accumulate<W8, COLS>(acc[0], w[0], xs, f);
                 if (second.slot >= 0) {
-                    if (r == r_begin && second.block == 0) ask(second.slot + 2);
                     tokens_of(xs, second);
                     factors_of(f, second, r);
                     accumulate<W8, COLS>(acc[0], w[1], xs, f);
