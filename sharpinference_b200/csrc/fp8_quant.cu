@@ -15,15 +15,13 @@ namespace {
 template <typename T> struct Piece;                      // 16 bytes of input
 template <> struct Piece<float> {
     static constexpr int N = 4;
-    static __device__ __forceinline__ void load(const float* p, float (&v)[4]) {
-        const float4 x = *reinterpret_cast<const float4*>(p);
-        v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+    static __device__ __forceinline__ void open(const uint4& x, float (&v)[4]) {
+        v[0] = __uint_as_float(x.x); v[1] = __uint_as_float(x.y); v[2] = __uint_as_float(x.z); v[3] = __uint_as_float(x.w);
     }
 };
 template <> struct Piece<bf16> {
     static constexpr int N = 8;
-    static __device__ __forceinline__ void load(const bf16* p, float (&v)[8]) {
-        const uint4 x = *reinterpret_cast<const uint4*>(p);
+    static __device__ __forceinline__ void open(const uint4& x, float (&v)[8]) {
         const uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -33,18 +31,50 @@ template <> struct Piece<bf16> {
     }
 };
 
-// The elements k .. k + N - 1 of a row of K; zeros behind its end.  VEC: every piece that starts inside the row may be
-// read whole or is cut by the end (16-byte alignment of the row's start is given).
+// The elements k .. k + N - 1 of a row of K as they lie in memory; zeros behind its end.  They are opened when all of a thread's
+// pieces have been asked for: opening one waits for it.  VEC: rows start on 16 bytes.  Else the two aligned pieces that hold
+// the elements are read (the second only if the row reaches into it; what shares an aligned piece with an element can be
+// read) and shifted together:
 template <typename T, bool VEC>
-__device__ __forceinline__ void load_piece(const T* row, int k, int K, float (&v)[Piece<T>::N]) {
-    constexpr int N = Piece<T>::N;
-    if (VEC && k + N <= K) {
-        Piece<T>::load(row + k, v);
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = k + i < K ? to_float(row[k + i]) : 0.0f;
+struct Raw {
+    uint4 lo, hi;
+    __device__ __forceinline__ void ask(const T* row, int k, int K) {
+        lo = hi = make_uint4(0u, 0u, 0u, 0u);
+        if (k >= K) return;
+        if (VEC) {
+            lo = *reinterpret_cast<const uint4*>(row + k);
+        } else {
+            const uintptr_t at = reinterpret_cast<uintptr_t>(row + k), first = at & ~uintptr_t(15);
+            lo = *reinterpret_cast<const uint4*>(first);
+            if (first + 16 < min(reinterpret_cast<uintptr_t>(row + K), at + 16)) hi = *reinterpret_cast<const uint4*>(first + 16);
+        }
     }
-}
+    __device__ __forceinline__ void open(const T* row, int k, int K, float (&v)[Piece<T>::N]) const {
+        constexpr int N = Piece<T>::N;
+        uint4 x = lo;
+        if (!VEC) {
+            const int off = (int)(reinterpret_cast<uintptr_t>(row + k) & 15);
+            uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+            if (off & 8) {
+#pragma unroll
+                for (int i = 0; i < 6; ++i) w[i] = w[i + 2];
+            }
+            if (off & 4) {
+#pragma unroll
+                for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
+            }
+            const int bits = (off & 3) * 8;
+            x = make_uint4(__funnelshift_r(w[0], w[1], bits), __funnelshift_r(w[1], w[2], bits), __funnelshift_r(w[2], w[3], bits),
+                           __funnelshift_r(w[3], w[4], bits));
+        }
+        Piece<T>::open(x, v);
+        if (k + N > K) {
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                if (k + i >= K) v[i] = 0.0f;
+        }
+    }
+};
 
 template <int N>
 __device__ __forceinline__ uint32_t amax_of(const float (&v)[N]) {
@@ -65,42 +95,46 @@ __device__ __forceinline__ void store_piece(uint8_t* dst, int room, const float 
     else *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
 }
 
-constexpr int ROWS_WARPS = 8, ROWS_EACH = 4;
-
-// A warp takes 512 bytes of each of four neighbouring rows: one block (float32) or two (bfloat16) of each.
-template <typename T, bool VEC>
+constexpr int ROWS_WARPS = 8;
+// A warp takes 512 bytes of each of EACH neighbouring rows: one block (float32) or two (bfloat16) of each.  Few rows: one, which
+// is the shortest way from a load to a store; many: 64 (float32) or 128 bytes (bfloat16) in flight a thread.
+template <typename T, bool VEC, int EACH>
 __global__ void __launch_bounds__(ROWS_WARPS * 32)
 fp8_rows_kernel(const T* x, long long ldx, const int* rows, int M, int K, uint8_t* q, long long ldq, float* scale) {
     constexpr int N = Piece<T>::N, LANES = fp8::BLOCK / N, SIDE = 32 / LANES;
     pdl_wait();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int kb = (blockIdx.y * ROWS_WARPS + warp) * SIDE + lane / LANES;
-    const int k = kb * fp8::BLOCK + (lane % LANES) * N;
-    const long long row0 = (long long)blockIdx.x * ROWS_EACH;
-    float v[ROWS_EACH][N];
+    const int lane = threadIdx.x & 31;
+    const int kb = (blockIdx.y * (blockDim.x / 32) + (threadIdx.x >> 5)) * SIDE + lane / LANES, k = kb * fp8::BLOCK + (lane % LANES) * N;
+    const long long row0 = (long long)blockIdx.x * EACH;
+    Raw<T, VEC> raw[EACH];
+    const T* row[EACH];
 #pragma unroll
-    for (int r = 0; r < ROWS_EACH; ++r) {
+    for (int r = 0; r < EACH; ++r) {
         const long long m = min(row0 + r, (long long)M - 1);
-        load_piece<T, VEC>(x + (rows ? rows[m] : m) * ldx, k, K, v[r]);
+        row[r] = x + (rows ? rows[m] : m) * ldx;
     }
-    float s[ROWS_EACH];
 #pragma unroll
-    for (int r = 0; r < ROWS_EACH; ++r) {
-        uint32_t m = amax_of<N>(v[r]);
+    for (int r = 0; r < EACH; ++r) raw[r].ask(row[r], k, K);
+    float s[EACH];
+#pragma unroll
+    for (int r = 0; r < EACH; ++r) {
+        float v[N];
+        raw[r].open(row[r], k, K, v);
+        uint32_t m = amax_of<N>(v);
 #pragma unroll
         for (int o = LANES / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
         s[r] = fp8::scale_of(m);
+        if (row0 + r < M) store_piece<N>(q + (row0 + r) * ldq + k, (int)(ldq - k), v, 1.0f / s[r]);
     }
-#pragma unroll
-    for (int r = 0; r < ROWS_EACH; ++r)
-        if (row0 + r < M) store_piece<N>(q + (row0 + r) * ldq + k, (int)(ldq - k), v[r], 1.0f / s[r]);
     if (lane % LANES == 0 && kb * fp8::BLOCK < K) {
         float* dst = scale + (long long)kb * M + row0;
-        if (M % 4 == 0) {
-            *reinterpret_cast<float4*>(dst) = make_float4(s[0], s[1], s[2], s[3]);
+        if (EACH % 4 == 0 && M % 4 == 0) {               // (a multiple of four rows from here on)
+#pragma unroll
+            for (int r = 0; r + 3 < EACH; r += 4)
+                if (row0 + r < M) *reinterpret_cast<float4*>(dst + r) = make_float4(s[r], s[r + 1], s[r + 2], s[r + 3]);
         } else {
 #pragma unroll
-            for (int r = 0; r < ROWS_EACH; ++r)
+            for (int r = 0; r < EACH; ++r)
                 if (row0 + r < M) dst[r] = s[r];
         }
     }
@@ -118,20 +152,35 @@ fp8_weight_kernel(const T* w, int N_, int K, long long ldw, long long group, uin
     const int k = blockIdx.x * fp8::BLOCK + (threadIdx.x % LANES) * N;
     const int n0 = blockIdx.y * fp8::BLOCK + threadIdx.x / LANES;
     const T* src = w + blockIdx.z * group;
-    float v[EACH][N];
+    uint8_t* const dst = q + ((long long)blockIdx.z * N_) * ldq;
+    // A whole block of aligned rows stays in registers; blocks at the edges and rows that start anywhere are read again (from
+    // L1 and L2), which leaves room for more of them on an SM
+    const bool whole = VEC && (blockIdx.x + 1) * fp8::BLOCK <= K && (blockIdx.y + 1) * fp8::BLOCK <= N_;
+    uint4 kept[EACH];
     uint32_t m = 0;
+    if (whole) {
 #pragma unroll
-    for (int r = 0; r < EACH; ++r) {
-        const int n = n0 + r * SIDE;
-        if (n < N_) {
-            load_piece<T, VEC>(src + n * ldw, k, K, v[r]);
-        } else {
+        for (int r = 0; r < EACH; ++r) kept[r] = *reinterpret_cast<const uint4*>(src + (n0 + r * SIDE) * ldw + k);
 #pragma unroll
-            for (int i = 0; i < N; ++i) v[r][i] = 0.0f;
+        for (int r = 0; r < EACH; ++r) {
+            float v[N];
+            Piece<T>::open(kept[r], v);
+            m = max(m, amax_of<N>(v));
+        }
+    } else {
+#pragma unroll 1
+        for (int r0 = 0; r0 < EACH; r0 += 4) {
+            Raw<T, VEC> raw[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) raw[r].ask(src + (n0 + (r0 + r) * SIDE) * ldw, k, n0 + (r0 + r) * SIDE < N_ ? K : 0);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                float v[N];
+                raw[r].open(src + (n0 + (r0 + r) * SIDE) * ldw, k, n0 + (r0 + r) * SIDE < N_ ? K : 0, v);
+                m = max(m, amax_of<N>(v));
+            }
         }
     }
-#pragma unroll
-    for (int r = 0; r < EACH; ++r) m = max(m, amax_of<N>(v[r]));
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
     if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = m;
@@ -139,11 +188,27 @@ fp8_weight_kernel(const T* w, int N_, int K, long long ldw, long long group, uin
 #pragma unroll
     for (int i = 0; i < WEIGHT_THREADS / 32; ++i) m = max(m, part[i]);
     const float s = fp8::scale_of(m), inv = 1.0f / s;
-    uint8_t* dst = q + ((long long)blockIdx.z * N_) * ldq;
+    if (whole) {
 #pragma unroll
-    for (int r = 0; r < EACH; ++r) {
-        const int n = n0 + r * SIDE;
-        if (n < N_) store_piece<N>(dst + n * ldq + k, (int)(ldq - k), v[r], inv);
+        for (int r = 0; r < EACH; ++r) {
+            float v[N];
+            Piece<T>::open(kept[r], v);
+            store_piece<N>(dst + (n0 + r * SIDE) * ldq + k, N, v, inv);
+        }
+    } else {
+#pragma unroll 1
+        for (int r0 = 0; r0 < EACH; r0 += 4) {
+            Raw<T, VEC> raw[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) raw[r].ask(src + (n0 + (r0 + r) * SIDE) * ldw, k, n0 + (r0 + r) * SIDE < N_ ? K : 0);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int n = n0 + (r0 + r) * SIDE;
+                float v[N];
+                raw[r].open(src + n * ldw, k, n < N_ ? K : 0, v);
+                if (n < N_) store_piece<N>(dst + n * ldq + k, (int)(ldq - k), v, inv);
+            }
+        }
     }
     if (threadIdx.x == 0) scale[((long long)blockIdx.z * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x] = s;
 }
@@ -153,17 +218,25 @@ bool vectors(const void* x, long long ld, long long group) {
     return (reinterpret_cast<uintptr_t>(x) & 15) == 0 && ld * (long long)sizeof(T) % 16 == 0 && group * (long long)sizeof(T) % 16 == 0;
 }
 
+template <typename T, int EACH>
+int rows_launch(const T* x, long long ldx, const int* rows, int M, int K, uint8_t* q, long long ldq, float* scale, cudaStream_t stream) {
+    constexpr int SIDE = 32 / (fp8::BLOCK / Piece<T>::N);
+    // a CTA's warps lie along K, as evenly as up to eight come
+    const int groups = (K + SIDE * fp8::BLOCK - 1) / (SIDE * fp8::BLOCK), along = (groups + ROWS_WARPS - 1) / ROWS_WARPS;
+    const int threads = 32 * ((groups + along - 1) / along);
+    const dim3 grid((M + EACH - 1) / EACH, along);
+    if (along > 65535) return SHARPI_BAD_ARGUMENT;
+    if (vectors<T>(x, ldx, 0)) SHARPI_LAUNCH_PDL((fp8_rows_kernel<T, true, EACH>), grid, threads, 0, stream, x, ldx, rows, M, K, q, ldq, scale);
+    else SHARPI_LAUNCH_PDL((fp8_rows_kernel<T, false, EACH>), grid, threads, 0, stream, x, ldx, rows, M, K, q, ldq, scale);
+    return SHARPI_OK;
+}
+
 template <typename T>
 int rows_impl(const void* x, long long ldx, const int* rows, int M, int K, void* q, long long ldq, float* scale, cudaStream_t stream) {
-    constexpr int SIDE = 32 / (fp8::BLOCK / Piece<T>::N);
-    const int blocks = (K + fp8::BLOCK - 1) / fp8::BLOCK;
-    const dim3 grid((M + ROWS_EACH - 1) / ROWS_EACH, (blocks + ROWS_WARPS * SIDE - 1) / (ROWS_WARPS * SIDE));
-    if (grid.y > 65535) return SHARPI_BAD_ARGUMENT;
     const T* src = static_cast<const T*>(x);
     uint8_t* dst = static_cast<uint8_t*>(q);
-    if (vectors<T>(x, ldx, 0)) SHARPI_LAUNCH_PDL((fp8_rows_kernel<T, true>), grid, ROWS_WARPS * 32, 0, stream, src, ldx, rows, M, K, dst, ldq, scale);
-    else SHARPI_LAUNCH_PDL((fp8_rows_kernel<T, false>), grid, ROWS_WARPS * 32, 0, stream, src, ldx, rows, M, K, dst, ldq, scale);
-    return SHARPI_OK;
+    return M <= 64 ? rows_launch<T, 1>(src, ldx, rows, M, K, dst, ldq, scale, stream)
+                   : rows_launch<T, (sizeof(T) == 4 ? 4 : 8)>(src, ldx, rows, M, K, dst, ldq, scale, stream);
 }
 
 template <typename T>

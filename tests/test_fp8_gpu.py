@@ -396,3 +396,19 @@ def test_split_over_k_by_experts(ops, name, split):
     left = torch.ones(rows, dtype=torch.bool, device=DEV)
     left[there] = False
     assert (out[left] == 5.0).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_quantisation_of_rows_that_start_anywhere(ops, dtype):
+    """Every distance of a row's start from a 16-byte boundary, rows that end inside of one, at the end of their memory."""
+    step = 16 // torch.tensor([], dtype=dtype).element_size()
+    for off in range(step):
+        for K in (1, step, 125, 128, 131, 255, 263):
+            x = rnd(9, off + K, dtype=dtype, seed=off + K)
+            part = x[:, off:]                                  # ends where its memory ends
+            q, scale = ops.fp8_rows(part)
+            want_q, want_scale = rows_definition(part)
+            assert same(q, want_q) and torch.equal(scale, want_scale)
+            q, scale = ops.fp8_weight(part)
+            want_q, want_scale = ops.fp8_weight(torch.nn.functional.pad(part, (0, -K % 16))[:, :K])
+            assert same(q, want_q) and torch.equal(scale, want_scale)
