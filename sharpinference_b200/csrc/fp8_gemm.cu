@@ -606,10 +606,20 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
     }
 }
 
+// The shared memory that a kernel may take, set once a device
+template <typename K>
+bool allow_shared(K kernel, bool (&done)[64]) {
+    int device = 0;
+    if (cudaGetDevice(&device) != cudaSuccess || device >= 64) return false;
+    if (!done[device]) done[device] = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM) == cudaSuccess;
+    return done[device];
+}
+
 template <int MODE, bool SPLIT>
 int launch(const CUtensorMap& ma, const CUtensorMap& mw, const Params& p, int ctas, cudaStream_t stream) {
     const auto kernel = fp8_gemm_kernel<MODE, SPLIT>;
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM) != cudaSuccess) return SHARPI_LAUNCH_FAILED;
+    static bool done[64];
+    if (!allow_shared(kernel, done)) return SHARPI_LAUNCH_FAILED;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = ctas;
     cfg.blockDim = THREADS;

@@ -507,11 +507,13 @@ _status_words = {}
 
 def status_word(device) -> torch.Tensor:
     """The device word in which a tensor-core kernel records a wait that gave up (0 = none)."""
-    device = torch.device(device)
     w = _status_words.get(device)
     if w is None:
-        w = torch.zeros(1, dtype=torch.int32, device=device)
-        _status_words[device] = w
+        device = torch.device(device)
+        w = _status_words.get(device)
+        if w is None:
+            w = torch.zeros(1, dtype=torch.int32, device=device)
+            _status_words[device] = w
     return w
 
 
@@ -559,6 +561,9 @@ _sm_counts = {}
 
 def sm_count(device=None) -> int:
     """Streaming multiprocessors of the device (asked once)."""
+    n = _sm_counts.get(device) if device is not None else None
+    if n is not None:
+        return n
     device = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
     n = _sm_counts.get(device)
     if n is None:
@@ -2107,40 +2112,40 @@ def fp8_blocks(n: int) -> int:
     return (n + FP8_BLOCK - 1) // FP8_BLOCK
 
 
-def _here(*tensors) -> None:
-    """All tensors given (or None) lie on the current device, on whose stream the kernels are launched."""
+def _here(*tensors) -> int:
+    """The current device, on whose stream the kernels are launched; all tensors given (or None) must lie there."""
     here = torch._C._cuda_getDevice()
     for t in tensors:
         if t is not None and t.get_device() != here:
             raise KernelError(f"a tensor is on {t.device}, the current device is cuda:{here}")
+    return here
 
 
 def fp8_empty(shape: Sequence[int], device) -> torch.Tensor:
     """An e4m3 tensor whose rows start on 16-byte boundaries (the bytes between the rows are not set)."""
     K = shape[-1]
     if K % 16 == 0:
-        return torch.empty(shape, dtype=FP8, device=device)
-    return torch.empty((*shape[:-1], (K + 15) // 16 * 16), dtype=FP8, device=device)[..., :K]
+        return torch.empty(*shape, dtype=FP8, device=device)
+    return torch.empty(*shape[:-1], (K + 15) // 16 * 16, dtype=FP8, device=device)[..., :K]
 
 
-def _need_fp8(q: torch.Tensor, scale: torch.Tensor, name: str, dims: int, scale_shape) -> int:
-    """The bytes between two rows of an 8-bit operand; raises where the products do not take it."""
+def _need_fp8(q: torch.Tensor, scale: torch.Tensor, name: str, scale_shape: tuple) -> int:
+    """The bytes between two rows of an 8-bit operand ``[rows, K]`` or ``[E, rows, K]``; raises where the products do not take it."""
     if not q.is_cuda:
         raise KernelError(f"{name} must be a CUDA tensor (the engine has no CPU path); found device {q.device}")
-    if q.dtype != FP8:
+    if q.dtype is not FP8:
         raise KernelError(f"{name} must have dtype {FP8}, found {q.dtype}")
-    if q.dim() != dims:
-        raise KernelError(f"{name} must have {dims} dimensions, found shape {tuple(q.shape)}")
-    K = q.shape[-1]
-    ld = q.stride(-2) if q.shape[-2] > 1 else (K + 15) // 16 * 16
-    if (K > 1 and q.stride(-1) != 1) or ld < K or (dims == 3 and q.shape[0] > 1 and q.stride(0) != ld * q.shape[1]):
-        raise KernelError(f"the rows of {name} must be contiguous and equally far apart, found strides {q.stride()} for shape {tuple(q.shape)}")
+    shape, stride = q.shape, q.stride()
+    K = shape[-1]
+    ld = stride[-2] if shape[-2] > 1 else (K + 15) // 16 * 16
+    if (K > 1 and stride[-1] != 1) or ld < K or (len(shape) == 3 and shape[0] > 1 and stride[0] != ld * shape[1]):
+        raise KernelError(f"the rows of {name} must be contiguous and equally far apart, found strides {stride} for shape {tuple(shape)}")
     if ld % 16 or q.data_ptr() % 16:
         raise KernelError(f"the rows of {name} must start on 16-byte boundaries, as fp8_rows, fp8_weight and fp8_empty lay "
                           f"them; found rows {ld} bytes apart")
     _need(scale, f"{name}_scale", torch.float32)
-    if tuple(scale.shape) != tuple(scale_shape):
-        raise KernelError(f"{name}_scale is {tuple(scale.shape)}, expected {tuple(scale_shape)}")
+    if scale.shape != scale_shape:
+        raise KernelError(f"{name}_scale is {tuple(scale.shape)}, expected {scale_shape}")
     return ld
 
 
@@ -2154,15 +2159,16 @@ def fp8_rows(x: torch.Tensor, *, rows: Optional[torch.Tensor] = None):
         _need(rows, "rows", torch.int32)
         if rows.dim() != 1:
             raise KernelError(f"rows must have one dimension, found shape {tuple(rows.shape)}")
-    _here(x, rows)
+    here = _here(x, rows)
     T, K = x.shape
     M = T if rows is None else rows.numel()
     if K == 0 or (M > 0 and T == 0):
         raise KernelError(f"x is {tuple(x.shape)}: no elements to quantise")
-    q = fp8_empty((M, K), x.device)
-    scale = torch.empty((fp8_blocks(K), M), dtype=torch.float32, device=x.device)
-    check(kernel("sharpi_fp8_rows")(x.data_ptr(), dtype, ld, _ptr(rows), M, K, q.data_ptr(), (K + 15) // 16 * 16, scale.data_ptr(),
-                                    _stream()), "sharpi_fp8_rows")
+    device = x.device
+    q = fp8_empty((M, K), device)
+    scale = torch.empty((K + 127) // 128, M, dtype=torch.float32, device=device)
+    check(kernel("sharpi_fp8_rows")(x.data_ptr(), dtype, ld, None if rows is None else rows.data_ptr(), M, K, q.data_ptr(),
+                                    (K + 15) // 16 * 16, scale.data_ptr(), torch._C._cuda_getCurrentRawStream(here)), "sharpi_fp8_rows")
     return q, scale
 
 
@@ -2191,13 +2197,15 @@ _OUT_DTYPES = (torch.float32, torch.bfloat16)
 
 def _fp8_product(a, a_scale, w, w_scale, group_offsets, *, swiglu=False, out=None, out_scale=None, out_dtype=torch.float32,
                  out_rows=None, row_scale=None, scale_rows=None, bias=None, accumulate=False, split=0):
-    if a.dim() != 2 or w.dim() not in (2, 3) or a.shape[1] != w.shape[-1] or a.shape[1] == 0:
-        raise KernelError(f"inner sizes differ or shapes are not [rows, K] and [N, K] or [E, N, K]: a {tuple(a.shape)}, w {tuple(w.shape)}")
-    rows, K = a.shape
-    N, E = w.shape[-2], (w.shape[0] if w.dim() == 3 else 1)
-    lda = _need_fp8(a, a_scale, "a", 2, (fp8_blocks(K), rows))
-    ldw = _need_fp8(w, w_scale, "w", w.dim(), (*w.shape[:-2], fp8_blocks(N), fp8_blocks(K)))
-    if (group_offsets is None) != (w.dim() == 2):
+    a_shape, w_shape = a.shape, w.shape
+    if len(a_shape) != 2 or len(w_shape) not in (2, 3) or a_shape[1] != w_shape[-1] or a_shape[1] == 0:
+        raise KernelError(f"inner sizes differ or shapes are not [rows, K] and [N, K] or [E, N, K]: a {tuple(a_shape)}, w {tuple(w_shape)}")
+    rows, K = a_shape
+    N, E = w_shape[-2], (w_shape[0] if len(w_shape) == 3 else 1)
+    KB, NB = (K + 127) // 128, (N + 127) // 128
+    lda = _need_fp8(a, a_scale, "a", (KB, rows))
+    ldw = _need_fp8(w, w_scale, "w", (NB, KB) if len(w_shape) == 2 else (E, NB, KB))
+    if (group_offsets is None) != (len(w_shape) == 2):
         raise KernelError("group_offsets [E + 1] belong to weights [E, N, K], and weights [N, K] have none")
     if group_offsets is not None:
         _need(group_offsets, "group_offsets", torch.int32)
@@ -2226,21 +2234,21 @@ def _fp8_product(a, a_scale, w, w_scale, group_offsets, *, swiglu=False, out=Non
             raise KernelError("accumulate=True needs an output tensor to add to")
         if out_dtype not in _OUT_DTYPES:
             raise KernelError(f"out_dtype {out_dtype} is not one of {_OUT_DTYPES}")
-        out = torch.empty((rows, N), dtype=out_dtype, device=a.device)
+        out = torch.empty(rows, N, dtype=out_dtype, device=a.device)
     elif not swiglu:
         _need(out, "out")
         if out.dtype not in _OUT_DTYPES or (accumulate and out.dtype != torch.float32):
             raise KernelError(f"out must be float32{'' if accumulate else ' or bfloat16'}, found {out.dtype}")
         if out.dim() != 2 or out.shape[1] != N or (out_rows is None and out.shape[0] < rows):
             raise KernelError(f"out is {tuple(out.shape)} for a product of {rows} rows and {N} columns")
-    _here(a, a_scale, w, w_scale, group_offsets, out, out_rows, row_scale, scale_rows, bias)
+    here = _here(a, a_scale, w, w_scale, out, group_offsets, out_rows, row_scale, scale_rows, bias)
     if rows == 0 or N == 0 or E == 0:
         return out
     check(kernel("sharpi_fp8_gemm")(a.data_ptr(), lda, a_scale.data_ptr(), w.data_ptr(), ldw, w_scale.data_ptr(), _ptr(group_offsets),
                                     _ptr(out_rows), _ptr(row_scale), _ptr(scale_rows), _ptr(bias), out.data_ptr(),
                                     out.stride(0) if swiglu else 0, _ptr(out_scale), status_word(a.device).data_ptr(), rows, N, K, E,
-                                    int(swiglu), int(out.dtype == torch.bfloat16), int(accumulate), split, sm_count(a.device), _stream()),
-          "sharpi_fp8_gemm")
+                                    swiglu, out.dtype is torch.bfloat16, accumulate, split, sm_count(a.device),
+                                    torch._C._cuda_getCurrentRawStream(here)), "sharpi_fp8_gemm")
     return out
 
 
@@ -2282,7 +2290,7 @@ def fp8_swiglu(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale:
         gate_up = _fp8_product(a, a_scale, w, w_scale, group_offsets, row_scale=row_scale, scale_rows=scale_rows)
         return fp8_rows(swiglu(gate_up, torch.float32))
     q = fp8_empty((rows, I), a.device)
-    scale = torch.empty((I // FP8_BLOCK, rows), dtype=torch.float32, device=a.device)
+    scale = torch.empty(I // FP8_BLOCK, rows, dtype=torch.float32, device=a.device)
     _fp8_product(a, a_scale, w, w_scale, group_offsets, swiglu=True, out=q, out_scale=scale, row_scale=row_scale, scale_rows=scale_rows)
     return q, scale
 
@@ -2335,8 +2343,8 @@ def moe_few(h: torch.Tensor, router_weight: torch.Tensor, gate_up: torch.Tensor,
     if w8 != (down_scale is not None):
         raise KernelError("gate_up and down both have scales or neither has")
     if w8:
-        ldg = _need_fp8(gate_up, gate_up_scale, "gate_up", 3, (E, fp8_blocks(2 * I), fp8_blocks(H)))
-        ldd = _need_fp8(down, down_scale, "down", 3, (E, fp8_blocks(H), fp8_blocks(I)))
+        ldg = _need_fp8(gate_up, gate_up_scale, "gate_up", (E, fp8_blocks(2 * I), fp8_blocks(H)))
+        ldd = _need_fp8(down, down_scale, "down", (E, fp8_blocks(H), fp8_blocks(I)))
         if I % 2:
             raise KernelError(f"the experts' width must be even, found {I}")
     else:
@@ -2363,7 +2371,7 @@ def moe_few(h: torch.Tensor, router_weight: torch.Tensor, gate_up: torch.Tensor,
     if out is None:
         if out_dtype not in _OUT_DTYPES:
             raise KernelError(f"out_dtype {out_dtype} is not one of {_OUT_DTYPES}")
-        out = torch.empty((T, H), dtype=out_dtype, device=h.device)
+        out = torch.empty(T, H, dtype=out_dtype, device=h.device)
     else:
         _need(out, "out")
         if out.dtype not in _OUT_DTYPES or tuple(out.shape) != (T, H):

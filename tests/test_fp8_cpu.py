@@ -29,6 +29,7 @@ def calls(monkeypatch):
 
     monkeypatch.setattr(ops, "kernel", kernel)
     monkeypatch.setattr(ops, "_stream", lambda: 0)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda index: 0, raising=False)
     monkeypatch.setattr(ops, "sm_count", lambda device=None: 148)
     monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: -1, raising=False)     # the CPU's index
     empty = torch.empty
