@@ -13,7 +13,7 @@
 // (128 lanes), each with half of the columns, a row and 128 sums a thread; one warp issues the copies, one the MMAs, two
 // multiply the scales of rows and weights into a ring in shared memory (a factor a row and weight tile), so the readers' loop
 // is loads from tensor memory and paired multiply-adds with one factor.  The registers go where the sums are (setmaxnreg: 2 x
-// 224 + 56).  4096 x 16384 x 5120: 338 us; sixteen readers with 64 sums each (104 registers, which spill) 356; with the operands
+// 224 + 56).  4096 x 16384 x 5120: 330 us; sixteen readers with 64 sums each (104 registers, which spill) 356; with the operands
 // swapped (weight rows on the lanes, a factor a column) 650 to 920.
 //
 // Two grids.  Many tiles: one CTA an SM that walks tiles of all experts, those of one weight tile one after the other; copies
@@ -22,7 +22,10 @@
 //
 // Two epilogues:
 //   MODE_STORE   C[out_row, n] = (or +=) s D + bias   float32 or bfloat16; out_row = out_rows[sorted row] or the sorted row,
-//                s = row_scale[scale_rows[sorted row] or sorted row] or 1
+//                s = row_scale[scale_rows[sorted row] or sorted row] or 1.  Where rows of C start on 32 bytes a thread stores its
+//                row, a sector a store; elsewhere sixteen columns at a time change hands in shared memory.  4096 x 16384 x 512:
+//                float32 94 us, bfloat16 65 (all rows through shared memory, two columns of sectors at a time: 107 and 73);
+//                16380 columns 98, 16383 columns 153
 //   MODE_SWIGLU  w holds gate rows [0, I) and up rows [I, 2 I), I a multiple of 128; h = silu(s g) * (s u) leaves in 8 bits:
 //                a tile's 128 columns of h are one block of the next product's K
 //
@@ -43,7 +46,7 @@ constexpr int READERS = 8;           // warps that read tensor memory
 constexpr int THREADS = 32 * (READERS + 4);
 constexpr int A_BYTES = BM * BK, W_BYTES = WN * BK, STAGE = A_BYTES + 2 * W_BYTES, STAGES = 4;
 constexpr int RING = 8;              // blocks of scale factors, [2][BM] floats each
-constexpr int STAGING = READERS * 1024;
+constexpr int STAGING = READERS * 32 * 16 * 4;
 constexpr int BARRIERS = 2 * STAGES + 4 + 2 * RING + 1;
 constexpr int SMEM = STAGES * STAGE + RING * 2 * BM * 4 + STAGING + BARRIERS * 8 + 16 + 1024;
 constexpr int MAX_SPLIT = 8;
@@ -65,7 +68,7 @@ struct Params {
     int rows, N, E, NB, KB;          // NB, KB: blocks of 128 along N and K
     int a_box;                       // rows of an activation copy
     int split;                       // CTAs of a cluster, each with its part of K
-    int out_bf16, accumulate, vec;   // vec: rows of out start on 16 bytes
+    int out_bf16, accumulate, vec;   // vec: the boundary on which rows of out start: 32, 16 or 0 (less)
 };
 
 __device__ __forceinline__ uint32_t instr_desc_e4m3(int m, int n) {  // e4m3 x e4m3 -> fp32, operands K-major
@@ -209,14 +212,21 @@ __device__ __forceinline__ float row_factor(const Params& p, int row) {
     return p.row_scale ? p.row_scale[p.scale_rows ? p.scale_rows[row] : row] : 1.0f;
 }
 
+// 32 bytes to a 32-byte boundary
+__device__ __forceinline__ void store_32(void* to, const uint32_t (&w)[8]) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]),
+                 "r"(w[5]), "r"(w[6]), "r"(w[7])
+                 : "memory");
+}
+
 template <int MODE, bool SPLIT>
 __global__ void __launch_bounds__(THREADS, 1)
 fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w, const Params p) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     float* ring = reinterpret_cast<float*>(smem + STAGES * STAGE);                        // [RING][2][BM]
-    uint8_t* staging = reinterpret_cast<uint8_t*>(ring + RING * 2 * BM);
-    uint64_t* full = reinterpret_cast<uint64_t*>(staging + STAGING);
+    float* staging = ring + RING * 2 * BM;                                                // [READERS][32][16]
+    uint64_t* full = reinterpret_cast<uint64_t*>(staging + READERS * 32 * 16);
     uint64_t* empty = full + STAGES;
     uint64_t* acc_full = empty + STAGES;
     uint64_t* acc_empty = acc_full + 2;
@@ -368,6 +378,9 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
             if (tile.group < 0) break;
             const int row = tile.row0 + at;
             const bool live = at < tile.rows;
+            // asked for here, in front of the tile's blocks, not when their sums wait for them
+            const float rs = live && !SPLIT ? row_factor(p, row) : 0.0f;
+            const int to = live && !SPLIT ? (MODE == MODE_STORE && p.out_rows ? p.out_rows[row] : row) : -1;
             float acc[2][64];
 #pragma unroll
             for (int i = 0; i < 64; ++i) acc[0][i] = acc[1][i] = 0.0f;
@@ -425,8 +438,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
                 break;
             }
             if (MODE == MODE_STORE && !ok) break;
-            const float rs = live ? row_factor(p, row) : 0.0f;
-            uint8_t* mine = staging + warp * 1024;
+            float* mine = staging + warp * 32 * 16;
             if constexpr (MODE == MODE_SWIGLU) {
                 // 64 columns of h a thread; the block's maximum over the two parts
                 uint32_t* peak = reinterpret_cast<uint32_t*>(staging) + turn * BM * 2 + at * 2;
@@ -456,86 +468,70 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
                     if (part == 0) p.out_scale[(size_t)tile.nt * p.rows + row] = s;
                 }
             } else {
-                // 32 bytes of every row at a time go through the warp's staging, so that a store writes whole sectors
-                const int to = live ? (p.out_rows ? p.out_rows[row] : row) : -1;
                 const int c0 = tile.nt * BN + part * WN;
-                const int flip = (lane >> 2) & 1;
-                auto put16 = [&](int piece, uint4 v) { *reinterpret_cast<uint4*>(mine + lane * 32 + ((piece ^ flip) * 16)) = v; };
-                auto get16 = [&](int i) {                             // 16 bytes of row i * 16 + lane / 2
-                    const int r = i * 16 + (lane >> 1);
-                    return *reinterpret_cast<const uint4*>(mine + r * 32 + (((lane & 1) ^ ((r >> 2) & 1)) * 16));
-                };
+                if (p.row_scale) {
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    if (p.row_scale) {
+                    for (int i = 0; i < WN; ++i) acc[i / 64][i % 64] *= rs;
+                }
+                if (p.bias) {
 #pragma unroll
-                        for (int i = 0; i < 64; ++i) acc[h][i] *= rs;
-                    }
-                    if (p.bias) {
-#pragma unroll
-                        for (int i = 0; i < 64; ++i) acc[h][i] += c0 + h * 64 + i < p.N ? p.bias[c0 + h * 64 + i] : 0.0f;
-                    }
+                    for (int i = 0; i < WN; ++i) acc[i / 64][i % 64] += c0 + i < p.N ? p.bias[c0 + i] : 0.0f;
+                }
+                if (p.vec == 32 && !p.accumulate) {
+                    // a row a thread, 32 bytes (a whole sector) at a time
                     if (p.out_bf16) {
-                        bf16* out = static_cast<bf16*>(p.out);
+                        bf16* dst = static_cast<bf16*>(p.out) + (size_t)to * p.N + c0;
 #pragma unroll
-                        for (int c = 0; c < 64; c += 16) {
+                        for (int i = 0; i < WN; i += 16) {
+                            uint32_t w[8];
 #pragma unroll
-                            for (int o = 0; o < 2; ++o) {
-                                uint32_t w[4];
-#pragma unroll
-                                for (int j = 0; j < 4; ++j) {
-                                    const __nv_bfloat162 two = __floats2bfloat162_rn(acc[h][c + o * 8 + j * 2], acc[h][c + o * 8 + j * 2 + 1]);
-                                    w[j] = *reinterpret_cast<const uint32_t*>(&two);
-                                }
-                                put16(o, make_uint4(w[0], w[1], w[2], w[3]));
+                            for (int j = 0; j < 8; ++j) {
+                                const __nv_bfloat162 two = __floats2bfloat162_rn(acc[i / 64][i % 64 + 2 * j], acc[i / 64][i % 64 + 2 * j + 1]);
+                                w[j] = *reinterpret_cast<const uint32_t*>(&two);
                             }
-                            __syncwarp();
-#pragma unroll
-                            for (int i = 0; i < 2; ++i) {
-                                const int r = __shfl_sync(0xffffffffu, to, i * 16 + (lane >> 1));
-                                const uint4 v = get16(i);
-                                const int n = c0 + h * 64 + c + (lane & 1) * 8;
-                                if (r < 0 || n >= p.N) continue;
-                                bf16* dst = out + (size_t)r * p.N + n;
-                                if (p.vec && n + 8 <= p.N) {
-                                    *reinterpret_cast<uint4*>(dst) = v;
-                                } else {
-                                    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                                    for (int j = 0; j < 8; ++j)
-                                        if (n + j < p.N) reinterpret_cast<unsigned short*>(dst)[j] = (unsigned short)(w[j / 2] >> (16 * (j & 1)));
-                                }
-                            }
-                            __syncwarp();
+                            if (live && c0 + i < p.N) store_32(dst + i, w);
                         }
                     } else {
-                        float* out = static_cast<float*>(p.out);
+                        float* dst = static_cast<float*>(p.out) + (size_t)to * p.N + c0;
 #pragma unroll
-                        for (int c = 0; c < 64; c += 8) {
+                        for (int i = 0; i < WN; i += 8) {
+                            uint32_t w[8];
 #pragma unroll
-                            for (int o = 0; o < 2; ++o) {
-                                const float* x = &acc[h][c + o * 4];
-                                put16(o, make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3])));
-                            }
-                            __syncwarp();
-#pragma unroll
-                            for (int i = 0; i < 2; ++i) {
-                                const int r = __shfl_sync(0xffffffffu, to, i * 16 + (lane >> 1));
-                                const uint4 v = get16(i);
-                                const int n = c0 + h * 64 + c + (lane & 1) * 4;
-                                if (r < 0 || n >= p.N) continue;
-                                float* dst = out + (size_t)r * p.N + n;
-                                const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-                                if (p.vec && !p.accumulate && n + 4 <= p.N) {
-                                    *reinterpret_cast<uint4*>(dst) = v;
-                                } else {
-#pragma unroll
-                                    for (int j = 0; j < 4; ++j)
-                                        if (n + j < p.N) put(p, (size_t)r * p.N + n + j, __uint_as_float(w[j]));
-                                }
-                            }
-                            __syncwarp();
+                            for (int j = 0; j < 8; ++j) w[j] = __float_as_uint(acc[i / 64][i % 64 + j]);
+                            if (live && c0 + i < p.N) store_32(dst + i, w);
                         }
+                    }
+                } else {
+                    // rows that start elsewhere, or sums that are added: sixteen columns of every row at a time through the warp's
+                    // staging (the pieces of a row swapped by two bits of it), so that neighbouring columns are neighbouring lanes'
+                    const int have = min(32, tile.rows - (warp & 3) * 32);
+#pragma unroll
+                    for (int c = 0; c < WN; c += 16) {
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) {
+                            const float* x = &acc[c / 64][c % 64 + q * 4];
+                            *reinterpret_cast<float4*>(mine + lane * 16 + (q ^ ((lane >> 1) & 3)) * 4) = make_float4(x[0], x[1], x[2], x[3]);
+                        }
+                        __syncwarp();
+                        if (p.vec && !p.accumulate) {
+#pragma unroll
+                            for (int r0 = 0; r0 < 32; r0 += 8) {
+                                const int r = r0 + (lane >> 2), n = c0 + c + (lane & 3) * 4, from = __shfl_sync(0xffffffffu, to, r);
+                                if (r >= have || n >= p.N) continue;
+                                const float4 v = *reinterpret_cast<const float4*>(mine + r * 16 + ((lane ^ (r >> 1)) & 3) * 4);
+                                const float x[4] = {v.x, v.y, v.z, v.w};
+                                if (p.out_bf16) store_four(static_cast<bf16*>(p.out) + (size_t)from * p.N + n, x);
+                                else store_four(static_cast<float*>(p.out) + (size_t)from * p.N + n, x);
+                            }
+                        } else {
+#pragma unroll 4
+                            for (int r0 = 0; r0 < have; r0 += 2) {
+                                const int r = r0 + (lane >> 4), n = c0 + c + (lane & 15), from = __shfl_sync(0xffffffffu, to, r);
+                                if (r < have && n < p.N)
+                                    put(p, (size_t)from * p.N + n, mine[r * 16 + ((((lane & 15) / 4) ^ (r >> 1)) & 3) * 4 + lane % 4]);
+                            }
+                        }
+                        __syncwarp();
                     }
                 }
             }
@@ -722,7 +718,8 @@ SHARPI_API int sharpi_fp8_gemm(const void* a, long long lda, const float* a_scal
     p.KB = (K + BK - 1) / BK;
     p.out_bf16 = out_bf16;
     p.accumulate = accumulate;
-    p.vec = (reinterpret_cast<uintptr_t>(out) & 15) == 0 && N % (out_bf16 ? 8 : 4) == 0;
+    const uintptr_t starts = reinterpret_cast<uintptr_t>(out) | (uintptr_t)N * (out_bf16 ? 2 : 4);
+    p.vec = starts % 32 == 0 ? 32 : starts % 16 == 0 ? 16 : 0;
     const long long row_tiles = rows < E ? rows : (rows + BM - 1) / BM + (E > 1 ? E : 0);        // at most
     const long long tiles = row_tiles * (swiglu ? N / BN : (N + BN - 1) / BN);
     if (tiles > 0x3fffffff / MAX_SPLIT) return SHARPI_BAD_ARGUMENT;

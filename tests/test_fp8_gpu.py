@@ -373,6 +373,26 @@ def test_split_over_k(ops, split, M, N, K):
     close(out, want + base.to(F64), err + (want.abs() + base.abs()) * 2.0 ** -23)
 
 
+@pytest.mark.parametrize("out_dtype", [F32, BF16])
+@pytest.mark.parametrize("start", [0, 8, 4, 1])
+@pytest.mark.parametrize("N", [272, 264, 260, 261, 24, 4])
+def test_outputs_on_every_boundary(ops, N, start, out_dtype):
+    """Rows of the output that start on 32, 16 or fewer bytes, few and many of them; what lies around them stays."""
+    K = 200
+    for M in (3, 41, 140):
+        t = operands(ops, M, N, K, seed=M + N)
+        want, S = product(*t)
+        around = torch.full((start + M * N + 64,), 7.0, dtype=out_dtype, device=DEV)
+        out = around[start:start + M * N].view(M, N)
+        ops._fp8_product(*t, None, split=1, out=out)
+        close(out, want, product_error(K, S))
+        assert (around[:start] == 7.0).all() and (around[start + M * N:] == 7.0).all()
+        if out_dtype == F32:
+            plain = out.clone()
+            ops._fp8_product(*t, None, split=1, out=out, accumulate=True)
+            assert torch.equal(out, plain + plain)
+
+
 @pytest.mark.parametrize("split", [1, 3, 8])
 @pytest.mark.parametrize("name", ["empty_experts", "over_a_tile", "rows_behind"])
 def test_split_over_k_by_experts(ops, name, split):
