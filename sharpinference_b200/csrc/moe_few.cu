@@ -15,12 +15,14 @@
 // in warp order: a call's result is the same every time, but the order (float32 rounding) of a token's sum goes by which
 // experts the whole call reaches.
 //
-// bfloat16 weights: mma.sync m16n8k16, act rounded to bfloat16 (2^-9 of its value) as in the other bfloat16 mixtures.
+// bfloat16 weights: mma.sync m16n8k16.  act is two bfloat16, its rounding and what that left (together within 2^-16 of its
+// value), multiplied one after the other into the same sums.  With the first alone (2^-8) a layer in bfloat16 is off by 1.4 times
+// its own rounding; the second costs 27.8 us for 27.0 (one token, 8 of 128 experts, 2048 x 768) and 163 for 145 (16 tokens).
 //
 // e4m3 weights with a scale for 128 x 128 (fp8.cuh): an e4m3 value is a float16 one (cvt, two an instruction), and the MMA is
 // m16n8k16 on float16.  (mma.sync on e4m3 is no instruction of this GPU's: it converts both operands for every tile, 1000
 // instructions a step of 4 KB where this takes 250.)  The activations are float16 times a power of two s for 128 neighbours such
-// that |x / s| < 2^15: of h's eight bits none is lost down to 2^-32 of its block's largest value, act is off by 2^-12 of its
+// that |x / s| < 2^15: of h's eight bits none is lost down to 2^-32 of its block's largest value, act is off by 2^-11 of its
 // value.  A block's 128 products are added in float32, then scaled and added.  Infinities and NaN make a block's scale NaN.
 //
 // The barrier needs all CTAs on the GPU at once: the launch is cooperative.  Its counters lie in the call's own workspace and
@@ -47,6 +49,7 @@ struct Params {
     const float* down_scale;      // e4m3: [E, blocks of H, blocks of I]
     const float* add;             // [T, H] or null
     void* act;                    // bf16 weights: bf16 [active, T, Ip]; e4m3: float [active, T, Ip]
+    bf16* act_low;                // bf16 weights: what act's rounding left, [active, T, Ip]
     __half* act16;                // e4m3: act / act_scale [active, T, Ip]
     float* act_scale;             // e4m3: [active, T, blocks of I]
     void* out;                    // [T, H]
@@ -610,7 +613,12 @@ moe_few_kernel(const Params p) {
                     if (!p.on_input) h *= weight;
                     const size_t at = ((size_t)unit.x * p.T + t) * p.Ip + col;
                     if constexpr (W8) static_cast<float*>(p.act)[at] = h;
-                    else static_cast<bf16*>(p.act)[at] = __float2bfloat16_rn(h);
+                    else {
+                        const bf16 high = __float2bfloat16_rn(h);
+                        const float v = __bfloat162float(high);
+                        static_cast<bf16*>(p.act)[at] = high;
+                        p.act_low[at] = __float2bfloat16_rn(fabsf(v) < INFINITY ? h - v : 0.0f);
+                    }
                 }
             }
         }
@@ -690,7 +698,7 @@ moe_few_kernel(const Params p) {
     }
     const uint8_t* const act = W8 ? reinterpret_cast<const uint8_t*>(p.act16) : static_cast<const uint8_t*>(p.act);
     // the tokens' elements of an item, and what its products are multiplied by in the rows from r on
-    auto tokens_of = [&](Tokens<W8> (&xs)[COLS], const Item& i) {
+    auto tokens_of = [&](Tokens<W8> (&xs)[COLS], const uint8_t* act, const Item& i) {
         const unsigned m = sm.mask[i.slot];
 #pragma unroll
         for (int n = 0; n < COLS; ++n) {
@@ -714,30 +722,37 @@ moe_few_kernel(const Params p) {
                 }
         }
     };
+    const uint8_t* const low = reinterpret_cast<const uint8_t*>(p.act_low);
+    auto add = [&](float (&sums)[COLS][4], const uint4 (&tile)[2][2], const Tokens<W8> (&xs)[COLS], const Tokens<W8> (&rest)[COLS], const Factors<COLS>& f) {
+        accumulate<W8, COLS>(sums, tile, xs, f);
+        if constexpr (!W8) multiply<W8, COLS>(sums, tile, rest);
+    };
     for (int r = r_begin, rows; r < r_end; r += rows) {
         const bool pair = two;
         rows = pair ? 32 : 16;
         clear();
         for (at = 0; at * WARPS + warp < items;) {
-            Tokens<W8> xs[COLS];
+            Tokens<W8> xs[COLS], rest[COLS];                              // (rest: bf16 weights)
             Factors<COLS> f;
             const Item first = item[0], second = item[1];
-            tokens_of(xs, first);
+            tokens_of(xs, act, first);
+            if constexpr (!W8) tokens_of(rest, low, first);
             factors_of(f, first, r);
             if (pair) {
-                accumulate<W8, COLS>(acc[0], w[0], xs, f);
+                add(acc[0], w[0], xs, rest, f);
                 if constexpr (W8) {
                     f.row[0] = p.down_scale[((unsigned)sm.expert[first.slot] * NB + (unsigned)min(r + 16 + g, p.H - 1) / fp8::BLOCK) * (unsigned)KB + first.block];
                     f.row[1] = p.down_scale[((unsigned)sm.expert[first.slot] * NB + (unsigned)min(r + 24 + g, p.H - 1) / fp8::BLOCK) * (unsigned)KB + first.block];
                 }
-                accumulate<W8, COLS>(acc[1], w[1], xs, f);
+                add(acc[1], w[1], xs, rest, f);
                 ++at;
             } else {
-                accumulate<W8, COLS>(acc[0], w[0], xs, f);
+                add(acc[0], w[0], xs, rest, f);
                 if (second.slot >= 0) {
-                    tokens_of(xs, second);
+                    tokens_of(xs, act, second);
+                    if constexpr (!W8) tokens_of(rest, low, second);
                     factors_of(f, second, r);
-                    accumulate<W8, COLS>(acc[0], w[1], xs, f);
+                    add(acc[0], w[1], xs, rest, f);
                 }
                 at += 2;
             }
@@ -827,6 +842,7 @@ SHARPI_API int sharpi_moe_few(const void* x, int x_dtype, int ldx, const void* h
     p.act = take(slots * T * Ip * (w8 ? 4 : 2));
     __half* rows16 = nullptr;
     float* x_scale = nullptr;
+    if (!w8) p.act_low = reinterpret_cast<bf16*>(take(slots * T * Ip * 2));
     if (w8) {
         p.act16 = reinterpret_cast<__half*>(take(slots * T * Ip * 2));
         p.act_scale = reinterpret_cast<float*>(take(slots * T * (Ip / 128) * 4));

@@ -2324,8 +2324,8 @@ def moe_few(h: torch.Tensor, router_weight: torch.Tensor, gate_up: torch.Tensor,
     :func:`fp8_weight` and an even ``I``.  ``weights_on``: a weight multiplies its expert's ``"input"`` (before the nonlinearity) or
     ``"output"``.  ``add`` float32 ``[T, H]`` is added (a shared expert's output; ``out`` may be it).
 
-    ``silu(g) * u`` is rounded to bfloat16 between the products, everything else is float32.  The order in which a token's terms
-    are added goes by the experts that the whole call reaches."""
+    Between the products ``silu(g) * u`` is two bfloat16 (2^-16 of its value), or (e4m3 weights) float16 times a power of two for
+    128 neighbours (2^-11); sums are float32.  The order in which a token's terms are added goes by the experts that the whole call reaches."""
     _need(h, "h", torch.bfloat16)
     _need(router_weight, "router_weight", torch.float32)
     if h.dim() != 2 or router_weight.dim() != 2 or gate_up.dim() != 3 or down.dim() != 3:
@@ -2382,7 +2382,7 @@ def moe_few(h: torch.Tensor, router_weight: torch.Tensor, gate_up: torch.Tensor,
     x = h if h32 is None else h32
     # the router's logits, silu(g) u of every (expert, token), the barrier's counters; with 8-bit weights activations in pieces
     slots, inner, wide = min(E, T * k), fp8_blocks(I) * FP8_BLOCK, fp8_blocks(H)
-    size = 64 + 4 * T * E + slots * T * inner * (6 if w8 else 2) + (4 * slots * T * (inner // FP8_BLOCK) + T * wide * (2 * FP8_BLOCK + 4) if w8 else 0) + 96
+    size = 64 + 4 * T * E + slots * T * inner * (6 if w8 else 4) + (4 * slots * T * (inner // FP8_BLOCK) + T * wide * (2 * FP8_BLOCK + 4) if w8 else 0) + 96
     work = torch.empty(size, dtype=torch.uint8, device=h.device)
     check(kernel("sharpi_moe_few")(x.data_ptr(), dtype_code(x.dtype), H, h.data_ptr(), H, router_weight.data_ptr(), _ptr(bias),
                                    _ptr(correction), gate_up.data_ptr(), ldg, _ptr(gate_up_scale), down.data_ptr(), ldd, _ptr(down_scale),
