@@ -147,10 +147,14 @@ __device__ __forceinline__ float4 peer_float4(uint32_t here, int rank) {
     return v;
 }
 
-// silu(g) * u with the exponential and the reciprocal as single instructions (relative error about 2^-21, before a
-// rounding to 2^-4); a large negative g gives -0 * u.
+// silu(g) * u.  The exponential and the reciprocal are single instructions; what rounding the exponent -g log2(e) leaves (2^x
+// is off by x 2^-24 ln 2 of its value otherwise) is a factor behind it, and a Newton step sharpens the reciprocal: an error
+// here sends a value to the next e4m3 number.  A large negative g gives -0 * u.
 __device__ __forceinline__ float silu_mul(float g, float u) {
-    return g * rcp_approx(1.0f + ex2_approx(-1.4426950408889634f * g)) * u;
+    const float x = -1.4426950408889634f * g, left = fmaf(-1.4426950408889634f, g, -x) - 1.925963033e-8f * g;
+    const bool plain = fabsf(x) < 120.0f;
+    const float e = ex2_approx(x), d = 1.0f + (plain ? fmaf(e, 0.6931471806f * left, e) : e), r = rcp_approx(d);
+    return g * (plain ? fmaf(r, fmaf(-d, r, 1.0f), r) : r) * u;
 }
 
 struct Tile {

@@ -279,6 +279,27 @@ def test_swiglu_dense(ops, M, I):
     check_swiglu(*ops.fp8_swiglu(*t), *product(*t), 520, torch.ones(1, 1, dtype=F64, device=DEV))
 
 
+@pytest.mark.parametrize("split", [1, 2])
+def test_silu_of_known_gates(ops, split):
+    """Every block of h is one number, silu of a float32 that the product has exactly, so the block's scale shows silu's error: the
+    exponential 2^-22, the reciprocal and the two sums 2^-22 together, the products and 1 / 448 another 2^-22."""
+    g = torch.cat([torch.linspace(-82, 82, 83), torch.tensor([1e-3, -1e-3, 0.3, 1.0 / 3])]).to(F32)
+    n = g.numel()
+    a, w = ops.fp8_empty((3, 256), DEV), ops.fp8_empty((2 * n * BLOCK, 256), DEV)
+    a.view(torch.uint8).zero_()
+    w.view(torch.uint8).zero_()
+    a[:, 0] = torch.ones(3, device=DEV).to(E4M3)
+    w[:, 0] = torch.ones(2 * n * BLOCK, device=DEV).to(E4M3)
+    a_scale, w_scale = torch.ones(2, 3, device=DEV), torch.ones(2 * n, 2, device=DEV)
+    w_scale[:n] = g.to(DEV).unsqueeze(1)
+    q, scale = ops.fp8_empty((3, n * BLOCK), DEV), torch.empty(n, 3, device=DEV)
+    ops._fp8_product(a, a_scale, w, w_scale, None, swiglu=True, out=q, out_scale=scale, split=split)
+    h = g.to(F64) * torch.sigmoid(g.to(F64))
+    least = 448 * 2.0 ** -126                           # the smallest scale, which a block of zeros has (the gate 0: 448 * 2^-126 - 0)
+    assert ((scale.to(F64).cpu() * 448 - h.abs().unsqueeze(1)).abs() <= h.abs().unsqueeze(1) * 3 * 2.0 ** -22 + least * (h == 0).unsqueeze(1)).all()
+    assert (q.to(F64).cpu().abs() == 448 * (h != 0).repeat_interleave(BLOCK)).all()
+
+
 def test_a_row_does_not_depend_on_the_rest(ops):
     """A row's bits are the same alone and among others of its kind of step, as in the other tensor-core kernels."""
     N, K = 512, 1024
