@@ -22,6 +22,8 @@
     python bench_kernels.py delta --batch 64 --tokens 1            (delta rule and its gated norm; --batch 1 --tokens 2048)
     python bench_kernels.py delta_prep --tokens 2048               (convolution, unit norms, steps, low-rank columns)
     python bench_kernels.py sandwich --tokens 2048                 (normed update and norm, side gate, element gate, router)
+    python bench_kernels.py fp8 --op grouped --rows 2048           (block-scaled 8-bit operators: rows, weight, dense, grouped, swiglu)
+    python bench_kernels.py moe_few --tokens 8 --weights e4m3      (a whole mixture layer for a few tokens)
     python bench_kernels.py elementwise --op add_rmsnorm_pair --tokens 2048 --hidden 2048
     python bench_kernels.py elementwise --op add_layernorm --tokens 2048 --hidden 2048
 
@@ -742,6 +744,71 @@ def attention_keys_prefill(ns) -> None:
           f"{2.0 * (d + dv) * nq * pairs / ms / 1e9:.0f} TFLOP/s")
 
 
+def _rotate(sets, call):
+    """A function that calls with the next of the sets each time, so that a call's inputs are not in the L2 cache."""
+    at = [0]
+
+    def fn():
+        at[0] = (at[0] + 1) % len(sets)
+        return call(sets[at[0]])
+    return fn
+
+
+def fp8(ns) -> None:
+    """The block-scaled 8-bit operators.  ``--rows`` activations against ``--n`` x ``--k`` weights (``swiglu``: ``--n`` is gate and up
+    rows together), dealt evenly to ``--experts`` for grouped and swiglu (0: dense)."""
+    M, N, K, E = ns.rows, ns.n, ns.k, ns.experts if ns.op in ("grouped", "swiglu") else 0
+    if ns.op == "rows":
+        sets = [torch.randn(M, K, device=DEV).to(torch.bfloat16) for _ in range(max(1, (256 << 20) // (M * K * 2)) if M * K > 1 << 20 else 4)]
+        call, nbytes, flops = ops.fp8_rows, M * K * 3, 0
+    elif ns.op == "weight":
+        sets = [torch.randn(N, K, device=DEV).to(torch.bfloat16) for _ in range(max(1, min(8, (256 << 20) // (N * K * 2))))]
+        call, nbytes, flops = ops.fp8_weight, N * K * 3, 0
+    else:
+        groups = max(E, 1)
+        offsets = torch.tensor([M * e // groups for e in range(groups + 1)], dtype=torch.int32, device=DEV) if E else None
+        reached = min(M, groups)
+        copies = max(1, min(8, (256 << 20) // (reached * N * K)))
+        sets = []
+        for _ in range(copies):
+            a = ops.fp8_rows(torch.randn(M, K, device=DEV))
+            w = ops.fp8_weight((torch.randn(groups * N, K, device=DEV, dtype=torch.bfloat16) * 0.02).view(*((groups, N, K) if E else (N, K))))
+            sets.append((*a, *w))
+        out = torch.empty(M, N, dtype=torch.bfloat16 if ns.out == "bfloat16" else torch.float32, device=DEV)
+        if ns.op == "swiglu":
+            call = lambda t: ops.fp8_swiglu(*t, offsets)
+        elif E:
+            call = lambda t: ops.fp8_grouped(*t, offsets, out=out)
+        else:
+            call = lambda t: ops.fp8_dense(*t, out=out)
+        written = M * (N // 2) if ns.op == "swiglu" else out.numel() * out.element_size()
+        nbytes, flops = reached * N * K + M * K + written, 2 * M * N * K
+    ms = _time(_rotate(sets, call), ns.iters)
+    shape = f"{M}x{K}" if ns.op == "rows" else f"{N}x{K}" if ns.op == "weight" else f"{M}x{N}x{K}" + (f", {E} experts" if E else "")
+    print(f"fp8 {ns.op} {shape}: {ms * 1e3:.1f} us, {nbytes / ms / 1e6:.0f} GB/s, {flops / ms / 1e9:.0f} TFLOP/s")
+
+
+def moe_few(ns) -> None:
+    T, E, k, H, I = ns.tokens, ns.experts, ns.top, ns.hidden, ns.inter
+    g = torch.Generator(device=DEV).manual_seed(0)
+    sets = []
+    for _ in range(2):
+        x = torch.empty(T, H, dtype=torch.bfloat16, device=DEV).normal_(generator=g)
+        router = torch.empty(E, H, device=DEV).normal_(0, H ** -0.5, generator=g)
+        gate_up = torch.empty(E, 2 * I, H, dtype=torch.bfloat16, device=DEV).normal_(0, H ** -0.5, generator=g)
+        down = torch.empty(E, H, I, dtype=torch.bfloat16, device=DEV).normal_(0, I ** -0.5, generator=g)
+        scales = {}
+        if ns.weights == "e4m3":
+            gate_up, scales["gate_up_scale"] = ops.fp8_weight(gate_up)
+            down, scales["down_scale"] = ops.fp8_weight(down)
+        reached = int(ops.router_topk(x.float(), router, k)[0].unique().numel())
+        sets.append((x, router, gate_up, down, scales, reached))
+    ms = _time(_rotate(sets, lambda s: ops.moe_few(*s[:4], k, **s[4])), ns.iters)
+    reached = sum(s[5] for s in sets) / len(sets)
+    nbytes = reached * 3 * I * H * sets[0][2].element_size() + E * H * 4
+    print(f"moe_few {ns.weights} tokens={T} top {k} of {E} ({reached:.0f} reached) {H}x{I}: {ms * 1e3:.1f} us, {nbytes / ms / 1e6:.0f} GB/s")
+
+
 def main(argv=None) -> int:
     ap = argparse.ArgumentParser(description=__doc__, formatter_class=argparse.RawDescriptionHelpFormatter)
     sub = ap.add_subparsers(dest="kernel", required=True)
@@ -900,6 +967,22 @@ def main(argv=None) -> int:
     p.add_argument("--experts", type=int, default=18)
     p.add_argument("--top", type=int, default=2)
     p.set_defaults(fn=softmax_mixture)
+    p = sub.add_parser("fp8")
+    p.add_argument("--op", choices=["rows", "weight", "dense", "grouped", "swiglu"], default="grouped")
+    p.add_argument("--rows", type=int, default=2048)
+    p.add_argument("--n", type=int, default=5120)
+    p.add_argument("--k", type=int, default=8192)
+    p.add_argument("--experts", type=int, default=16)
+    p.add_argument("--out", choices=["float32", "bfloat16"], default="float32")
+    p.set_defaults(fn=fp8)
+    p = sub.add_parser("moe_few")
+    p.add_argument("--tokens", type=int, default=1)
+    p.add_argument("--experts", type=int, default=128)
+    p.add_argument("--top", type=int, default=8)
+    p.add_argument("--hidden", type=int, default=2048)
+    p.add_argument("--inter", type=int, default=768)
+    p.add_argument("--weights", choices=["bfloat16", "e4m3"], default="bfloat16")
+    p.set_defaults(fn=moe_few)
     for sp in sub.choices.values():
         sp.add_argument("--iters", type=int, default=10)
         sp.add_argument("--graph", action="store_true", help="time replays of a CUDA graph of the calls")
