@@ -95,9 +95,11 @@ __device__ __forceinline__ void store_piece(uint8_t* dst, int room, const float 
     else *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
 }
 
-constexpr int ROWS_WARPS = 8;
-// A warp takes 512 bytes of each of EACH neighbouring rows: one block (float32) or two (bfloat16) of each.  Few rows: one, which
-// is the shortest way from a load to a store; many: 64 (float32) or 128 bytes (bfloat16) in flight a thread.
+constexpr int ROWS_WARPS = 8, FEW_BYTES = 10 << 20;
+// A warp takes 512 bytes of each of EACH neighbouring rows: one block (float32) or two (bfloat16) of each.  Up to 10 MB of x: one,
+// which is the shortest way from a load to a store; more: 64 (float32) or 128 bytes (bfloat16) in flight a thread.  Rows of 5120,
+// one against several, us: 8 MB 3.5 and 4.1 (float32), 4.0 and 5.8 (bfloat16); 16 MB 5.8 and 5.3, 6.7 and 6.6; 48 MB 15.5 and 12.5,
+// 18.2 and 15.3.
 template <typename T, bool VEC, int EACH>
 __global__ void __launch_bounds__(ROWS_WARPS * 32)
 fp8_rows_kernel(const T* x, long long ldx, const int* rows, int M, int K, uint8_t* q, long long ldq, float* scale) {
@@ -235,7 +237,7 @@ template <typename T>
 int rows_impl(const void* x, long long ldx, const int* rows, int M, int K, void* q, long long ldq, float* scale, cudaStream_t stream) {
     const T* src = static_cast<const T*>(x);
     uint8_t* dst = static_cast<uint8_t*>(q);
-    return M <= 64 ? rows_launch<T, 1>(src, ldx, rows, M, K, dst, ldq, scale, stream)
+    return (long long)M * K * (long long)sizeof(T) <= FEW_BYTES ? rows_launch<T, 1>(src, ldx, rows, M, K, dst, ldq, scale, stream)
                    : rows_launch<T, (sizeof(T) == 4 ? 4 : 8)>(src, ldx, rows, M, K, dst, ldq, scale, stream);
 }
 

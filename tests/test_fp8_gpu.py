@@ -56,6 +56,21 @@ def test_rows(ops, dtype, M, K):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("M,K", [(1400, 5120), (5500, 1003), (10007, 640), (11001, 520), (42000, 130)])
+def test_many_rows(ops, dtype, M, K):
+    """More than the 10 MB up to which a warp has one row at a time; row counts that are no multiple of what it has then."""
+    base = rnd(M, K + 5, dtype=dtype, scale=3.0, seed=K)
+    for x in (base[:, :K].contiguous(), base[:, 3:K + 3]):
+        q, scale = ops.fp8_rows(x)
+        want_q, want_scale = rows_definition(x)
+        assert same(q, want_q) and torch.equal(scale, want_scale)
+    at = torch.randperm(M, generator=torch.Generator().manual_seed(1))[: M - 3].to(torch.int32).to(DEV)
+    q, scale = ops.fp8_rows(base[:, :K], rows=at)
+    want_q, want_scale = rows_definition(base[at.long(), :K])
+    assert same(q, want_q) and torch.equal(scale, want_scale)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
 def test_rows_of_zeros_tiny_and_broken_numbers(ops, dtype):
     x = rnd(8, 384, dtype=dtype, seed=5)
     x[0] = 0.0
