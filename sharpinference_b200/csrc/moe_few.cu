@@ -9,7 +9,9 @@
 // pieces straight into registers.  Teams of 1 to 16 warps share K in turn (the more K has, the more); a warp asks for its next
 // step of 4 KB when it has multiplied the last (up to 64 KB an SM in flight; reading at 6.4 TB/s with a microsecond of latency
 // takes 44 KB; asking whole rows into L2 ahead of that took 3 to 8 % longer).  8 tokens, 1 of 16 experts of 5120 x 8192 in 8 bits:
-// 181 us, 4.5 TB/s.  Weights are the 16-row operand of the MMA (eight gate rows and their up rows, or sixteen rows of the down
+// 178 us, 4.6 TB/s.  The activations come through L1: a copy of them in shared memory left too little of it for the loads on
+// their way (2 of 16 experts, bfloat16: 16 tokens of 5120 118 us and 194 with the copy, 8 of 8192 103 and 116, 8 of 2048 the
+// same).  Weights are the 16-row operand of the MMA (eight gate rows and their up rows, or sixteen rows of the down
 // matrix), tokens the eight columns; a column of a token that did not choose the expert is computed and dropped (gate|up) or
 // zero (down).  Because the down product is linear, a token's experts are one long sum over
 // (expert, inner element): act is multiplied by the router's weight before (weights on the output).  The warps' parts are added
@@ -58,7 +60,7 @@ struct Params {
     int* status;
     long long ldg, ldd;           // bytes
     int ldx, T, E, k, H, I, Ip;   // Ip: I rounded up to 128
-    int softmax, renormalize, on_input, out_bf16, staged;      // staged: the rows x fit into shared memory
+    int softmax, renormalize, on_input, out_bf16;
     int team;                     // warps that share the K of gate and up rows
     float scale;
 };
@@ -416,22 +418,10 @@ moe_few_kernel(const Params p) {
     constexpr int SIZE = W8 ? 1 : 2;                                      // bytes of a weight
     constexpr int X_STEP = W8 ? 2 * STEP : STEP;                          // bytes of a step of a token's row
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
-    // rows x in shared memory: a pitch of 64 bytes over a multiple of 128 puts two rows' 64 bytes into different banks
-    const int pitch = (p.ldx + 127) / 128 * 128 + 64;
-    uint8_t* const staged = smem + sizeof(Shared) + scores_bytes(p.T, p.E);
     for (int e = threadIdx.x; e < p.E; e += THREADS) sm.users[e] = 0;
     if (threadIdx.x < 16) sm.zeros[threadIdx.x] = make_uint4(0u, 0u, 0u, 0u);
     __syncthreads();
     pdl_wait();
-    if (p.staged) {
-        const int each = p.ldx / 16;
-#pragma unroll 1
-        for (int r = warp; r < p.T; r += WARPS)
-#pragma unroll 4
-            for (int c = lane; c < each; c += 32) mma16::cp_async_16(staged + (size_t)r * pitch + c * 16, p.x + (size_t)r * p.ldx + c * 16, 16);
-    }
-    mma16::cp_async_commit();
-
     // ---- who goes where (every CTA for itself) ------------------------------------------------
     if (warp < p.T) choose(p, sm, rest + warp * p.E, warp);
     __syncthreads();
@@ -471,7 +461,6 @@ moe_few_kernel(const Params p) {
         const int a = sm.slot[sm.chosen[i]], t = i / p.k;
         sm.factor[sm.first[a] + __popc(sm.mask[a] & ((1u << t) - 1))] = sm.weight[i];
     }
-    mma16::cp_async_wait_all();
     __syncthreads();
     const int active = sm.active;
 
@@ -511,13 +500,11 @@ moe_few_kernel(const Params p) {
         const int team = p.team;
         const int me = warp % team, my_team = warp / team, teams = gridDim.x * (WARPS / team), index = blockIdx.x * (WARPS / team) + my_team;
         const int u_begin = (int)(units * index / teams), u_end = (int)(units * (index + 1) / teams);
-        const uint8_t* const x = p.staged ? staged : p.x;
-        const unsigned ld = p.staged ? pitch : p.ldx;
         const uint8_t* x_row[COLS];                                       // (a token there is not has another's row: it is dropped)
         const float* x_scale[COLS];
 #pragma unroll
         for (int n = 0; n < COLS; ++n) {
-            x_row[n] = x + min(8 * n + g, p.T - 1) * ld;
+            x_row[n] = p.x + min(8 * n + g, p.T - 1) * p.ldx;
             x_scale[n] = p.x_scale + min(8 * n + 2 * t4, p.T - 1) * KB;
         }
         const int odd[2] = {2 * t4 + 1 < p.T ? KB : 0, 8 + 2 * t4 + 1 < p.T ? KB : 0};
@@ -791,11 +778,7 @@ moe_few_kernel(const Params p) {
 template <bool W8, int COLS>
 int launch(Params& p, int sms, cudaStream_t stream) {
     const auto kernel = moe_few_kernel<W8, COLS>;
-    const size_t scores = scores_bytes(p.T, p.E);
-    const size_t rows = (size_t)p.T * ((p.ldx + 127) / 128 * 128 + 64);
-    constexpr size_t MOST = 226 * 1024;
-    p.staged = sizeof(Shared) + scores + rows <= MOST;
-    const size_t smem = sizeof(Shared) + scores + (p.staged ? rows : 0);
+    const size_t smem = sizeof(Shared) + scores_bytes(p.T, p.E);
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) return SHARPI_LAUNCH_FAILED;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = sms;
