@@ -78,7 +78,7 @@ def close(got, want, bound):
 @pytest.mark.parametrize("weights", ["bfloat16", "e4m3"])
 @pytest.mark.parametrize("T,E,k,H,I", [(1, 8, 2, 128, 64), (1, 128, 8, 2048, 768), (2, 3, 3, 1000, 40), (5, 16, 1, 520, 200), (8, 16, 4, 1024, 512),
                                        (9, 16, 2, 1024, 136), (16, 64, 8, 640, 384), (16, 4, 4, 256, 1000), (16, 300, 32, 128, 64),
-                                       (3, 1, 1, 64, 8)])
+                                       (3, 1, 1, 64, 8), (16, 1024, 32, 64, 8), (2, 4, 2, 8, 8), (16, 2, 1, 9008, 64), (13, 4, 2, 64, 2504)])
 def test_layer(ops, weights, T, E, k, H, I):
     c = layer(ops, T, E, H, I, weights, seed=T + E + H)
     for i, on in enumerate(("input", "output")):
@@ -190,6 +190,29 @@ def test_the_same_again_in_graphs_and_on_streams(ops, weights):
             side = call(ops, c, k)
     torch.cuda.synchronize()
     assert torch.equal(side, want) and all(torch.equal(o, want) for o in outs)
+
+
+def test_calls_side_by_side(ops):
+    """Layers on streams of two priorities at once, with a product that fills the GPU on a third: each layer's blocks wait for one
+    another, none for another launch's."""
+    E, k, H, I = 16, 4, 512, 256
+    layers = [layer(ops, T, E, H, I, seed=T) for T in (3, 12)]
+    want = [call(ops, c, k) for c in layers]
+    a, w = ops.fp8_rows(rnd(300, 1024, seed=1)), ops.fp8_weight(rnd(7168, 1024, seed=2))
+    product = ops.fp8_dense(*a, *w)
+    streams = [torch.cuda.Stream(priority=p) for p in (0, -1, -2)]
+    torch.cuda.synchronize()
+    got = [[], [], []]
+    for i in range(60):
+        for j, c in enumerate(layers):
+            with torch.cuda.stream(streams[j]):
+                got[j].append(call(ops, c, k))
+        if i % 3 == 0:
+            with torch.cuda.stream(streams[2]):
+                got[2].append(ops.fp8_dense(*a, *w))
+    torch.cuda.synchronize()
+    ops.check_status(DEV)
+    assert all(torch.equal(y, want[j]) for j in range(2) for y in got[j]) and all(torch.equal(y, product) for y in got[2])
 
 
 def test_beside_the_chain_of_kernels(ops):
