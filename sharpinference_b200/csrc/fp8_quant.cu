@@ -8,7 +8,7 @@
 // Rows of q are `ldq` bytes apart, a multiple of 16 (what a TMA copy of them needs); the bytes behind K are zeros.
 //
 // Both are bound by the bytes they move: a piece of 16 bytes stays in registers between the maximum and the rounding (a weight's
-// blocks at its edges are read again).  8192 x 5120 float32 35.8 us, 5.9 TB/s; bfloat16 23.8 us, 5.3; a weight of 7001 x 5112 18.7.  The
+// blocks at its edges are read again).  8192 x 5120 float32 35.8 us, 5.9 TB/s; bfloat16 23.5 us, 5.4; a weight of 7001 x 5112 18.7.  The
 // maximum of bfloat16 is taken two elements an instruction, on their bits.
 #include "fp8.cuh"
 
@@ -104,11 +104,11 @@ __device__ __forceinline__ void store_piece(uint8_t* dst, int room, const uint4&
     else *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
 }
 
-constexpr int ROWS_WARPS = 8, FEW_BYTES = 10 << 20;
-// A warp takes 512 bytes of each of EACH neighbouring rows: one block (float32) or two (bfloat16) of each.  Up to 10 MB of x: one,
-// which is the shortest way from a load to a store; more: 64 (float32) or 128 bytes (bfloat16) in flight a thread.  Rows of 5120,
-// one against several, us: 8 MB 3.5 and 4.1 (float32), 4.0 and 5.8 (bfloat16); 16 MB 5.8 and 5.3, 6.7 and 6.6; 48 MB 15.5 and 12.5,
-// 18.2 and 15.3.
+constexpr int ROWS_WARPS = 8, FEW_BYTES = 9 << 20;
+// A warp takes 512 bytes of each of EACH neighbouring rows: one block (float32) or two (bfloat16) of each.  Up to 9 MB of x: one,
+// which is the shortest way from a load to a store; more: four, 64 bytes in flight a thread.  Rows of 5120, one against four, us:
+// 6 MB 3.0 and 3.5 (float32), 3.2 and 4.0 (bfloat16); 12 MB 4.5 and 4.2, 5.2 and 5.0; 48 MB 15.5 and 12.5, 17.4 and 15.0.  (Eight rows
+// of bfloat16 2 to 11 % longer, 40 % where rows start anywhere.)
 template <typename T, bool VEC, int EACH>
 __global__ void __launch_bounds__(ROWS_WARPS * 32)
 fp8_rows_kernel(const T* x, long long ldx, const int* rows, int M, int K, uint8_t* q, long long ldq, float* scale) {
@@ -233,7 +233,7 @@ int rows_impl(const void* x, long long ldx, const int* rows, int M, int K, void*
     const T* src = static_cast<const T*>(x);
     uint8_t* dst = static_cast<uint8_t*>(q);
     return (long long)M * K * (long long)sizeof(T) <= FEW_BYTES ? rows_launch<T, 1>(src, ldx, rows, M, K, dst, ldq, scale, stream)
-                   : rows_launch<T, (sizeof(T) == 4 ? 4 : 8)>(src, ldx, rows, M, K, dst, ldq, scale, stream);
+                   : rows_launch<T, 4>(src, ldx, rows, M, K, dst, ldq, scale, stream);
 }
 
 template <typename T>

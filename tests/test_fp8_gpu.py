@@ -58,7 +58,7 @@ def test_rows(ops, dtype, M, K):
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("M,K", [(1400, 5120), (5500, 1003), (10007, 640), (11001, 520), (42000, 130)])
 def test_many_rows(ops, dtype, M, K):
-    """More than the 10 MB up to which a warp has one row at a time; row counts that are no multiple of what it has then."""
+    """More than the 9 MB up to which a warp has one row at a time; row counts that are no multiple of what it has then."""
     base = rnd(M, K + 5, dtype=dtype, scale=3.0, seed=K)
     for x in (base[:, :K].contiguous(), base[:, 3:K + 3]):
         q, scale = ops.fp8_rows(x)
