@@ -12,11 +12,12 @@
 // 178 us, 4.6 TB/s.  The activations come through L1: a copy of them in shared memory left too little of it for the loads on
 // their way (2 of 16 experts, bfloat16: 16 tokens of 5120 118 us and 194 with the copy, 8 of 8192 103 and 116, 8 of 2048 the
 // same).  Weights are the 16-row operand of the MMA (eight gate rows and their up rows, or sixteen rows of the down
-// matrix), tokens the eight columns; a column of a token that did not choose the expert is computed and dropped (gate|up) or
-// zero (down).  Because the down product is linear, a token's experts are one long sum over
-// (expert, inner element): act is multiplied by the router's weight before (weights on the output).  The warps' parts are added
-// in warp order: a call's result is the same every time, but the order (float32 rounding) of a token's sum goes by which
-// experts the whole call reaches.
+// matrix), tokens the eight columns; a column of a token that did not choose the expert is computed and dropped (gate|up), or is
+// zeros and its sums stay as they were (down: selected, not added, since 0 times an infinity or a NaN among the expert's weights
+// is a NaN; 9 to 16 tokens with bfloat16 weights take 1 to 4 % longer for it, the others nothing).  Because the down product is
+// linear, a token's experts are one long sum over (expert, inner element): act is multiplied by the router's weight before (weights
+// on the output).  The warps' parts are added in warp order: a call's result is the same every time, but the order (float32
+// rounding) of a token's sum goes by which experts the whole call reaches.
 //
 // bfloat16 weights: mma.sync m16n8k16.  act is two bfloat16, its rounding and what that left (together within 2^-16 of its
 // value), multiplied one after the other into the same sums.  With the first alone (2^-8) a layer in bfloat16 is off by 1.4 times
@@ -259,7 +260,8 @@ __device__ __forceinline__ void multiply(float (&sums)[COLS][4], const uint4 (&w
     }
 }
 
-// What a block's products are multiplied by (e4m3): the scales of rows g and g + 8 and of tokens 2 t and 2 t + 1
+// What a block's products are multiplied by (e4m3): the scales of rows g and g + 8 and of tokens 2 t and 2 t + 1 (0: a token that
+// did not choose the expert; a block's scale is 2^-126 at least)
 template <int COLS>
 struct Factors {
     float row[2], token[COLS][2];
@@ -278,7 +280,8 @@ __device__ __forceinline__ void accumulate(float (&acc)[COLS][4], const uint4 (&
 #pragma unroll
         for (int n = 0; n < COLS; ++n)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) acc[n][j] = fmaf(part[n][j], f.row[j / 2] * f.token[n][j % 2], acc[n][j]);
+            for (int j = 0; j < 4; ++j)
+                acc[n][j] = f.token[n][j % 2] != 0.0f ? fmaf(part[n][j], f.row[j / 2] * f.token[n][j % 2], acc[n][j]) : acc[n][j];
     } else {
         multiply<W8, COLS>(acc, w, x);
     }
@@ -711,9 +714,24 @@ moe_few_kernel(const Params p) {
         }
     };
     const uint8_t* const low = reinterpret_cast<const uint8_t*>(p.act_low);
-    auto add = [&](float (&sums)[COLS][4], const uint4 (&tile)[2][2], const Tokens<W8> (&xs)[COLS], const Tokens<W8> (&rest)[COLS], const Factors<COLS>& f) {
-        accumulate<W8, COLS>(sums, tile, xs, f);
-        if constexpr (!W8) multiply<W8, COLS>(sums, tile, rest);
+    auto add = [&](float (&sums)[COLS][4], const uint4 (&tile)[2][2], const Tokens<W8> (&xs)[COLS], const Tokens<W8> (&rest)[COLS], const Factors<COLS>& f,
+                   const Item& item) {
+        if constexpr (W8) {
+            accumulate<W8, COLS>(sums, tile, xs, f);
+        } else {
+            float next[COLS][4];
+#pragma unroll
+            for (int n = 0; n < COLS; ++n)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) next[n][j] = sums[n][j];
+            multiply<W8, COLS>(next, tile, xs);
+            multiply<W8, COLS>(next, tile, rest);
+            const unsigned m = sm.mask[item.slot] >> (2 * t4);
+#pragma unroll
+            for (int n = 0; n < COLS; ++n)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) sums[n][j] = m >> (8 * n + j % 2) & 1 ? next[n][j] : sums[n][j];
+        }
     };
     for (int r = r_begin, rows; r < r_end; r += rows) {
         const bool pair = two;
@@ -727,20 +745,20 @@ moe_few_kernel(const Params p) {
             if constexpr (!W8) tokens_of(rest, low, first);
             factors_of(f, first, r);
             if (pair) {
-                add(acc[0], w[0], xs, rest, f);
+                add(acc[0], w[0], xs, rest, f, first);
                 if constexpr (W8) {
                     f.row[0] = p.down_scale[((unsigned)sm.expert[first.slot] * NB + (unsigned)min(r + 16 + g, p.H - 1) / fp8::BLOCK) * (unsigned)KB + first.block];
                     f.row[1] = p.down_scale[((unsigned)sm.expert[first.slot] * NB + (unsigned)min(r + 24 + g, p.H - 1) / fp8::BLOCK) * (unsigned)KB + first.block];
                 }
-                add(acc[1], w[1], xs, rest, f);
+                add(acc[1], w[1], xs, rest, f, first);
                 ++at;
             } else {
-                add(acc[0], w[0], xs, rest, f);
+                add(acc[0], w[0], xs, rest, f, first);
                 if (second.slot >= 0) {
                     tokens_of(xs, act, second);
                     if constexpr (!W8) tokens_of(rest, low, second);
                     factors_of(f, second, r);
-                    add(acc[0], w[1], xs, rest, f);
+                    add(acc[0], w[1], xs, rest, f, second);
                 }
                 at += 2;
             }

@@ -145,6 +145,39 @@ def test_broken_numbers_stay_with_their_token(ops, weights):
     assert torch.equal(call(ops, c, k), whole)
 
 
+@pytest.mark.parametrize("weights,where", [("bfloat16", "element"), ("e4m3", "element"), ("e4m3", "scale")])
+@pytest.mark.parametrize("T,H,I", [(6, 256, 136), (13, 264, 128), (8, 5120, 200), (16, 2600, 264)])
+def test_broken_weights_stay_with_the_tokens_that_chose_their_expert(ops, weights, T, H, I, where):
+    """A NaN or an infinity in one expert's matrix: the other tokens' outputs are the bits that they are with whole weights."""
+    E, k = 8, 2
+    c = layer(ops, T, E, H, I, weights, seed=T)
+    whole = call(ops, c, k)
+    expert = ops.router_topk(c["h32"], c["router"], k)[0]
+    users = [(expert == e).any(1) for e in range(E)]
+    e = next(i for i in range(E) if 0 < int(users[i].sum()) < T)
+    mine, others = users[e], ~users[e]
+    for name, row in (("down", H - 3), ("down", 17), ("gate_up", I + 5), ("gate_up", 0)):
+        for value in (float("nan"), float("inf"), float("-inf")):
+            d = dict(c)
+            if where == "scale":
+                d[name + "_scale"] = c[name + "_scale"].clone()
+                d[name + "_scale"][e, row // 128, 0] = value
+            elif weights == "e4m3":
+                d[name] = ops.fp8_empty(c[name].shape, DEV).copy_(c[name])
+                d[name].view(torch.uint8)[e, row, 3] = 0x7f if value > 0 or value != value else 0xff      # e4m3 has NaN of both signs
+            else:
+                d[name] = c[name].clone()
+                d[name][e, row, 3] = value
+            y = call(ops, d, k)
+            assert torch.equal(y[others], whole[others])
+            if name == "down":                          # (one row of the matrix, or a scale's block of them, is one output element)
+                at = torch.arange(H, device=DEV)
+                hit = at // 128 == row // 128 if where == "scale" else at == row
+                assert not torch.isfinite(y[mine][:, hit]).any() and torch.equal(y[mine][:, ~hit], whole[mine][:, ~hit])
+            else:
+                assert not torch.isfinite(y[mine]).any()
+
+
 def test_weights_whose_rows_lie_apart(ops):
     T, E, H, I, k = 5, 6, 256, 128, 2
     c = layer(ops, T, E, H, I, seed=12)
