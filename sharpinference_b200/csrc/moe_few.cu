@@ -37,6 +37,7 @@
 namespace {
 
 constexpr int MAX_T = 16, MAX_K = 32, MAX_E = 1024;
+constexpr int IN_REGISTERS = 128;              // experts whose scores a warp holds in registers while it chooses
 constexpr int WARPS = 16, THREADS = 32 * WARPS;
 constexpr int NT = 2;                          // tiles of sixteen weight rows that a warp has at a time
 constexpr uint32_t BARRIER_LIMIT = 1u << 22;
@@ -330,7 +331,7 @@ __device__ __forceinline__ void choose(const Params& p, Shared& sm, uint32_t* re
         if (lane == j) mine = at;
         return at;
     };
-    if (p.E <= 128) {                                      // four a lane, in registers
+    if (p.E <= IN_REGISTERS) {                             // four a lane
         uint32_t key[4];
         float s[4];
 #pragma unroll
@@ -385,8 +386,8 @@ __device__ __forceinline__ void choose(const Params& p, Shared& sm, uint32_t* re
     if (lane < p.k) sm.weight[t * p.k + lane] = broken ? __int_as_float(0x7fc00000) : s * (p.softmax || p.renormalize ? p.scale / total : p.scale);
 }
 
-// Bytes of shared memory for the choice
-__host__ __device__ __forceinline__ size_t scores_bytes(int T, int E) { return ((size_t)T * E * 4 + 15) / 16 * 16; }
+// Bytes of shared memory for the scores of the choice (up to 128 experts: registers hold them)
+constexpr int scores_bytes(int T, int E) { return E <= IN_REGISTERS ? 0 : (T * E * 4 + 15) / 16 * 16; }
 
 // A barrier of `threads` threads of the CTA, a multiple of 32
 __device__ __forceinline__ void named_barrier(int id, int threads) {
@@ -417,7 +418,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 moe_few_kernel(const Params p) {
     extern __shared__ __align__(16) uint8_t smem[];
     Shared& sm = *reinterpret_cast<Shared*>(smem);
-    uint32_t* const rest = reinterpret_cast<uint32_t*>(smem + sizeof(Shared));      // [T, E]
+    uint32_t* const rest = reinterpret_cast<uint32_t*>(smem + sizeof(Shared));      // [T, E], or nothing
     constexpr int SIZE = W8 ? 1 : 2;                                      // bytes of a weight
     constexpr int X_STEP = W8 ? 2 * STEP : STEP;                          // bytes of a step of a token's row
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
@@ -793,15 +794,27 @@ moe_few_kernel(const Params p) {
     }
 }
 
+// The shared memory that a kernel may take, set once a device to what its largest call takes: the limit belongs to the
+// function, and calls of several sizes may be on their way from several threads
+template <typename K>
+bool allow_shared(K kernel, bool (&done)[64]) {
+    int device = 0;
+    if (cudaGetDevice(&device) != cudaSuccess || device >= 64) return false;
+    if (!done[device])
+        done[device] = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                            (int)sizeof(Shared) + scores_bytes(MAX_T, MAX_E)) == cudaSuccess;
+    return done[device];
+}
+
 template <bool W8, int COLS>
 int launch(Params& p, int sms, cudaStream_t stream) {
     const auto kernel = moe_few_kernel<W8, COLS>;
-    const size_t smem = sizeof(Shared) + scores_bytes(p.T, p.E);
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) return SHARPI_LAUNCH_FAILED;
+    static bool done[64];
+    if (!allow_shared(kernel, done)) return SHARPI_LAUNCH_FAILED;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = sms;
     cfg.blockDim = THREADS;
-    cfg.dynamicSmemBytes = smem;
+    cfg.dynamicSmemBytes = sizeof(Shared) + scores_bytes(p.T, p.E);
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeCooperative;

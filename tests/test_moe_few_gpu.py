@@ -248,6 +248,40 @@ def test_calls_side_by_side(ops):
     assert all(torch.equal(y, want[j]) for j in range(2) for y in got[j]) and all(torch.equal(y, product) for y in got[2])
 
 
+def test_calls_of_several_threads(ops, monkeypatch):
+    """Layers whose kernels take different amounts of shared memory, launched by four threads at once."""
+    import threading
+    layers = [(layer(ops, 8, 1024, 64, 8, seed=1), 32), (layer(ops, 1, 2, 64, 8, seed=2), 1)]
+    want = [call(ops, c, k) for c, k in layers]
+    # the launches alone, again and again: a call's arguments, and what it allocated kept alive
+    launch, empty, args, kept = ops.kernel("sharpi_moe_few"), torch.empty, [], []
+    streams = [torch.cuda.Stream() for _ in range(4)]
+    monkeypatch.setattr(torch, "empty", lambda *a, **k: kept.append(empty(*a, **k)) or kept[-1])
+    monkeypatch.setattr(ops, "kernel", lambda symbol: lambda *a: args.append(a) or 0)
+    got = []
+    for i, s in enumerate(streams):
+        with torch.cuda.stream(s):
+            c, k = layers[i % 2]
+            got.append(call(ops, c, k))
+    monkeypatch.undo()
+    torch.cuda.synchronize()
+    start, codes = threading.Barrier(4), [set() for _ in streams]
+
+    def work(i):
+        start.wait()
+        for _ in range(3000):
+            codes[i].add(launch(*args[i]))
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert codes == [{0}] * 4
+    assert all(torch.equal(y, want[i % 2]) for i, y in enumerate(got))
+
+
 def test_beside_the_chain_of_kernels(ops):
     """The same layer as the parts run it: one launch after the other over sorted rows, in bfloat16."""
     T, E, H, I, k = 8, 16, 512, 256, 2
