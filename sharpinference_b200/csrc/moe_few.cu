@@ -306,9 +306,9 @@ struct alignas(16) Shared {
 };
 static_assert(sizeof(Shared) % 16 == 0, "rows of 16-byte pieces lie behind it");
 
-// A float as a number in its order; NaN lowest
+// A float as a number in its order, the two zeros equal; NaN lowest
 __device__ __forceinline__ uint32_t order(float v) {
-    const uint32_t b = __float_as_uint(v);
+    const uint32_t b = __float_as_uint(v + 0.0f);          // (-0 + 0 = 0)
     return v == v ? (b & 0x80000000u ? ~b : b | 0x80000000u) : 0u;
 }
 

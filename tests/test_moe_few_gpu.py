@@ -115,6 +115,20 @@ def test_ties_go_to_the_lowest_index(ops):
     close(call(ops, c, 4), *plain(c, expert, torch.full((T, 4), 0.5, device=DEV), "output"))
 
 
+@pytest.mark.parametrize("E", [40, 300])
+def test_zeros_of_both_signs_are_a_tie(ops, E):
+    """Logits of -0 (products too small for float32 and a bias of -0) and of 0 are equal: the lowest indices are chosen."""
+    T, H, I = 3, 128, 64
+    c = layer(ops, T, E, H, I, seed=1)
+    c["h32"].fill_(1e-30)
+    c["router"].fill_(-1e-30)
+    c["router"][1::2] = 1e-30
+    bias = torch.full((E,), -0.0, device=DEV)
+    expert, weight, _ = ops.router_topk(c["h32"], c["router"], 4, scoring="softmax_chosen", bias=bias)
+    assert torch.equal(expert, torch.arange(4, device=DEV, dtype=torch.int32).repeat(T, 1))
+    close(call(ops, c, 4, scoring="softmax_chosen", bias=bias), *plain(c, expert, weight, "output"))
+
+
 def test_add_and_out(ops):
     T, E, H, I, k = 4, 8, 256, 128, 2
     c = layer(ops, T, E, H, I, seed=2)
