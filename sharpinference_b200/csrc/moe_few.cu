@@ -378,8 +378,8 @@ __device__ __forceinline__ void choose(const Params& p, Shared& sm, uint32_t* re
         atomicOr(&sm.users[mine], 1u << t);
         sm.chosen[t * p.k + lane] = mine;
     }
-    if (p.softmax) {                                       // the first choice has the largest logit
-        const float top = __shfl_sync(0xffffffffu, s, 0);
+    if (p.softmax) {                                       // (with a correction any of the chosen may have the largest logit)
+        const float top = warp_max(lane < p.k ? s : -INFINITY);
         s = lane < p.k ? expf(s - top) : 0.0f;
     }
     const float total = warp_sum(s);

@@ -147,7 +147,7 @@ router_topk_kernel(const float* __restrict__ h, const float* __restrict__ wr, co
             __syncwarp();
         }
     }
-    float total = 0.0f, top = 0.0f;
+    float total = 0.0f;
     int mine = 0;                                          // lane j keeps the j-th choice
     for (int j = 0; j < k; ++j) {
         float best = -INFINITY;
@@ -168,16 +168,14 @@ router_topk_kernel(const float* __restrict__ h, const float* __restrict__ wr, co
             c_s[at] = -INFINITY;
         }
         if (lane == j) mine = at;
-        if (scoring == 1) {                                // the first choice has the largest logit
-            if (j == 0) top = s_s[at];
-            total += expf(s_s[at] - top);
-        } else {
-            total += s_s[at];
-        }
+        if (scoring != 1) total += s_s[at];
         __syncwarp();
     }
-    if (scoring == 1) {
-        if (lane < k) weight[(size_t)t * k + lane] = expf(s_s[mine] - top) * (scale / total);
+    if (scoring == 1) {                                    // (with a correction any of the chosen may have the largest logit)
+        const float z = lane < k ? s_s[mine] : -INFINITY;
+        const float x = expf(z - warp_max(z));
+        for (int j = 0; j < k; ++j) total += __shfl_sync(0xffffffffu, x, j);
+        if (lane < k) weight[(size_t)t * k + lane] = x * (scale / total);
         return;
     }
     const float factor = renormalize ? scale / (scoring == 2 ? total + 1e-20f : total) : scale;

@@ -129,6 +129,25 @@ def test_zeros_of_both_signs_are_a_tie(ops, E):
     close(call(ops, c, 4, scoring="softmax_chosen", bias=bias), *plain(c, expert, weight, "output"))
 
 
+@pytest.mark.parametrize("E", [12, 300])
+def test_softmax_whose_largest_logit_is_not_the_first_choice(ops, E):
+    """A correction enters the choice alone: logits far above the first choice's are among the chosen."""
+    T, H, I, k = 3, 128, 64, 3
+    c = layer(ops, T, E, H, I, seed=3)
+    c["router"].zero_()
+    bias, correction = torch.zeros(E, device=DEV), torch.zeros(E, device=DEV)
+    bias[:4] = torch.tensor([0.0, 200.0, -5.0, 199.0], device=DEV)
+    correction[:4] = torch.tensor([2000.0, 1000.0, 0.0, 900.0], device=DEV)
+    chosen = torch.tensor([0, 1, 3], dtype=torch.int32, device=DEV)
+    weight = torch.softmax(bias[chosen.long()].to(F64), 0)
+    expert, got, _ = ops.router_topk(c["h32"], c["router"], k, scoring="softmax_chosen", bias=bias, correction=correction)
+    assert torch.equal(expert, chosen.repeat(T, 1))
+    assert ((got.to(F64) - weight).abs() <= weight * 2.0 ** -20 + 2.0 ** -126).all()       # (exp(-200) is 0 in float32)
+    y = call(ops, c, k, scoring="softmax_chosen", bias=bias, correction=correction)
+    want, bound = plain(c, expert, weight.repeat(T, 1), "output")
+    close(y, want, bound + want.abs() * 2.0 ** -20)     # the weights: exponentials and a quotient of float32
+
+
 def test_add_and_out(ops):
     T, E, H, I, k = 4, 8, 256, 128, 2
     c = layer(ops, T, E, H, I, seed=2)
