@@ -65,6 +65,7 @@ struct Params {
     int softmax, renormalize, on_input, out_bf16;
     int team;                     // warps that share the K of gate and up rows
     float scale;
+    uint32_t polls;               // of a barrier's counter before a wait gives up
 };
 
 // The scale of a block whose largest magnitude has the bits `amax`: a power of two such that amax / s < 2^15
@@ -396,13 +397,13 @@ __device__ __forceinline__ void named_barrier(int id, int threads) {
 }
 
 // Every thread of the grid behind every other's stores.  False: gave up.
-__device__ __forceinline__ bool grid_barrier(int* counter, int* go) {
+__device__ __forceinline__ bool grid_barrier(int* counter, int* go, uint32_t polls) {
     __syncthreads();
     if (threadIdx.x == 0) {
         __threadfence();
         atomicAdd(counter, 1);
         int seen = 0;
-        for (uint32_t i = 0; i < BARRIER_LIMIT && !seen; ++i) {
+        for (uint32_t i = 0; i < polls && !seen; ++i) {
             int v;
             asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(v) : "l"(counter) : "memory");
             seen = v >= (int)gridDim.x;
@@ -661,7 +662,7 @@ moe_few_kernel(const Params p) {
         two = r_end - r0 > 16;
         fetch_items();
     }
-    bool met = grid_barrier(p.barrier, &sm.go);
+    bool met = grid_barrier(p.barrier, &sm.go, p.polls);
     if constexpr (W8) {
         // act in float16, a warp a (slot, token, block)
         if (met) {
@@ -681,7 +682,7 @@ moe_few_kernel(const Params p) {
                 *reinterpret_cast<uint2*>(p.act16 + (size_t)r * p.Ip + col) = halves(v, s);
                 if (lane == 0) p.act_scale[(size_t)r * KB + b] = s;
             }
-            met = grid_barrier(p.barrier + 1, &sm.go);
+            met = grid_barrier(p.barrier + 1, &sm.go, p.polls);
         }
     }
     if (!met) {
@@ -826,7 +827,13 @@ int launch(Params& p, int sms, cudaStream_t stream) {
     return cudaLaunchKernelEx(&cfg, kernel, p) == cudaSuccess ? SHARPI_OK : SHARPI_LAUNCH_FAILED;
 }
 
+uint32_t test_polls = BARRIER_LIMIT;
+
 }  // namespace
+
+// Test hook: the waits of the NEXT launch poll `polls` times at most (0: every block gives up at once, writes the code and
+// returns).
+SHARPI_API void sharpi_moe_few_set_wait_test(unsigned polls) { test_polls = polls; }
 
 // h bf16 [T, H] rows ldh elements apart (bf16 weights: ldh a multiple of 8, 16-byte alignment), x: what the router reads,
 // float32 or bfloat16 [T, ldx]; weights bf16, or e4m3 with scales; rows ldg / ldd bytes apart; work: 16-byte aligned.
@@ -881,6 +888,8 @@ SHARPI_API int sharpi_moe_few(const void* x, int x_dtype, int ldx, const void* h
     p.add = add; p.out = out; p.status = status;
     p.ldg = ldg; p.ldd = ldd;
     p.T = T; p.E = E; p.k = k; p.H = H; p.I = I; p.Ip = Ip;
+    p.polls = test_polls;
+    test_polls = BARRIER_LIMIT;
     p.softmax = softmax; p.renormalize = renormalize; p.on_input = on_input; p.out_bf16 = out_bf16; p.scale = scale;
     // As many warps a team as leave each of them four steps of a row's K, so that joining their sums stays a small part; where the
     // teams then have 20 units and more, whose count no longer has to come out even, half as many.  Four steps against eight: 1 to

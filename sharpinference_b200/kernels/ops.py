@@ -2298,6 +2298,16 @@ def fp8_swiglu(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale:
 MOE_FEW_TOKENS = 16
 
 
+def moe_few_set_wait_test(polls: int) -> None:
+    """Test hook: the blocks of the next ``moe_few`` launch poll for one another at most ``polls`` times, so that with 0 the
+    wait runs out, the kernel records its code in the status word and returns; ``check_status`` then raises."""
+    import ctypes
+    from .library import load_library
+    fn = load_library("moe_few").sharpi_moe_few_set_wait_test
+    fn.argtypes, fn.restype = [ctypes.c_uint], None
+    fn(int(polls))
+
+
 def _need_rows_16(w: torch.Tensor, name: str) -> int:
     """Bytes between the rows of a weight ``[E, N, K]``, which start on 16-byte boundaries."""
     size = w.element_size()

@@ -338,3 +338,19 @@ def test_a_barrier_that_is_not_reached_is_reported(ops):
     with pytest.raises(ops.KernelError, match="19"):
         ops.check_status(DEV)
     ops.check_status(DEV)
+
+
+@pytest.mark.parametrize("weights", ["bfloat16", "e4m3"])
+@pytest.mark.parametrize("T", [3, 12])
+def test_a_wait_for_other_blocks_that_runs_out(ops, weights, T):
+    """The blocks of one launch poll for one another not once: the kernel records its code and returns, and the next call is right."""
+    c = layer(ops, T, 8, 256, 128, weights, seed=T)
+    want = call(ops, c, 2)
+    ops.check_status(DEV)
+    ops.moe_few_set_wait_test(0)
+    call(ops, c, 2)
+    with pytest.raises(ops.KernelError, match="code 19"):
+        ops.check_status(DEV)
+    ops.check_status(DEV)                               # the word is back at zero
+    assert torch.equal(call(ops, c, 2), want)
+    ops.check_status(DEV)
