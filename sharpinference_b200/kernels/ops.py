@@ -2195,6 +2195,15 @@ def fp8_weight(w: torch.Tensor):
 _OUT_DTYPES = (torch.float32, torch.bfloat16)
 
 
+def fp8_set_wait_test() -> None:
+    """Test hook: the next 8-bit product loads nothing behind the first block of K and polls each wait a few thousand times at most,
+    so a wait runs out, the kernel records its code in the status word and returns; ``check_status`` then raises."""
+    from .library import load_library
+    fn = load_library("fp8_gemm").sharpi_fp8_set_wait_test
+    fn.argtypes, fn.restype = [], None
+    fn()
+
+
 def _fp8_product(a, a_scale, w, w_scale, group_offsets, *, swiglu=False, out=None, out_scale=None, out_dtype=torch.float32,
                  out_rows=None, row_scale=None, scale_rows=None, bias=None, accumulate=False, split=0):
     a_shape, w_shape = a.shape, w.shape

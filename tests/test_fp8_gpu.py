@@ -468,3 +468,29 @@ def test_quantisation_of_rows_that_start_anywhere(ops, dtype):
             q, scale = ops.fp8_weight(part)
             want_q, want_scale = ops.fp8_weight(torch.nn.functional.pad(part, (0, -K % 16))[:, :K])
             assert same(q, want_q) and torch.equal(scale, want_scale)
+
+
+@pytest.mark.parametrize("swiglu", [False, True])
+@pytest.mark.parametrize("split", [1, 3])
+def test_a_wait_that_runs_out_is_reported_and_the_kernel_returns(ops, split, swiglu):
+    """One launch loads nothing behind the first block of K and polls each wait a few thousand times: a wait runs out, the kernel
+    records a code and returns (no fault, no hang), check_status raises it, and the next launch is right again."""
+    M, I, K = 300, 256, 1100
+    t = operands(ops, M, 2 * I, K, seed=M)
+
+    def product_of():
+        out = ops.fp8_empty((M, I), DEV) if swiglu else torch.empty(M, 2 * I, device=DEV)
+        scale = torch.empty(blocks(I), M, device=DEV)
+        ops._fp8_product(*t, None, split=split, out=out, **(dict(swiglu=True, out_scale=scale) if swiglu else {}))
+        return out, scale
+
+    want = product_of()
+    ops.check_status(DEV)
+    ops.fp8_set_wait_test()
+    product_of()
+    with pytest.raises(ops.KernelError, match="gave up"):
+        ops.check_status(DEV)
+    ops.check_status(DEV)                               # the word is back at zero
+    got = product_of()
+    ops.check_status(DEV)
+    assert same(got[0], want[0]) and (not swiglu or torch.equal(got[1], want[1]))
