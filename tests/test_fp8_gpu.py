@@ -315,6 +315,56 @@ def test_silu_of_known_gates(ops, split):
     assert (q.to(F64).cpu().abs() == 448 * (h != 0).repeat_interleave(BLOCK)).all()
 
 
+def ragged(rows_up_to, E, seed):
+    """Offsets of experts with no, a few, and many rows: tiles whose last warps have no rows before and behind full ones."""
+    g = torch.Generator().manual_seed(seed)
+    counts = torch.randint(1, rows_up_to, (E,), generator=g)
+    counts[torch.randperm(E, generator=g)[: E // 5]] = 0
+    counts[torch.randperm(E, generator=g)[: E // 3]] = torch.randint(1, 32, (E // 3,), generator=g)
+    offsets = torch.zeros(E + 1, dtype=torch.int32)
+    offsets[1:] = counts.cumsum(0)
+    return offsets.to(DEV), int(offsets[-1])
+
+
+# hundreds of tiles more than the GPU has SMs, so that a CTA walks several: blocks of K odd and even in number, one alone; rows of C
+# that start on 32 bytes, 16 and fewer
+@pytest.mark.parametrize("out_dtype", [F32, BF16])
+@pytest.mark.parametrize("M,N,K", [(2700, 5200, 300), (2689, 5203, 512), (2561, 5128, 100), (5000, 2600, 1000)])
+def test_dense_walk_over_many_tiles(ops, out_dtype, M, N, K):
+    t = operands(ops, M, N, K, seed=M)
+    want, S = product(*t)
+    close(ops._fp8_product(*t, None, split=1, out_dtype=out_dtype), want, product_error(K, S))
+
+
+@pytest.mark.parametrize("out_dtype", [F32, BF16])
+@pytest.mark.parametrize("E,N,K,most", [(60, 1040, 384, 200), (90, 1033, 520, 150), (40, 2072, 128, 600)])
+def test_grouped_walk_over_many_tiles(ops, out_dtype, E, N, K, most):
+    offsets, rows = ragged(most, E, seed=E)
+    assert rows > E and (N + 255) // 256 * int(((offsets.diff() + 127) // 128).sum()) > 2 * 148
+    t = operands(ops, rows, N, K, E=E, seed=E)
+    want, S = product(*t, offsets)
+    to = torch.randperm(rows + 9, generator=torch.Generator().manual_seed(1))[:rows].to(torch.int32).to(DEV)
+    weight = rnd(rows + 9, seed=2)
+    out = torch.full((rows + 9, N), 5.0, dtype=out_dtype, device=DEV)
+    ops._fp8_product(*t, offsets, split=1, out=out, out_rows=to, row_scale=weight, scale_rows=to)
+    s = weight[to.long()].to(F64).unsqueeze(1)
+    close(out[to.long()], want * s, (product_error(K, S) + want.abs() * 2.0 ** -24) * s.abs())
+    left = torch.ones(rows + 9, dtype=torch.bool, device=DEV)
+    left[to.long()] = False
+    assert (out[left] == 5.0).all()
+
+
+@pytest.mark.parametrize("E,I,K,most", [(40, 1280, 256, 300), (60, 768, 392, 200), (30, 2048, 100, 500)])
+def test_swiglu_walk_over_many_tiles(ops, E, I, K, most):
+    offsets, rows = ragged(most, E, seed=E + 1)
+    assert I // 128 * int(((offsets.diff() + 127) // 128).sum()) > 2 * 148
+    t = operands(ops, rows, 2 * I, K, E=E, seed=E)
+    weight = rnd(rows, seed=4).abs()
+    q, scale = ops.fp8_empty((rows, I), DEV), torch.empty(blocks(I), rows, device=DEV)
+    ops._fp8_product(*t, offsets, swiglu=True, out=q, out_scale=scale, row_scale=weight, split=1)
+    check_swiglu(q, scale, *product(*t, offsets), K, weight.to(F64).unsqueeze(1))
+
+
 def test_a_row_does_not_depend_on_the_rest(ops):
     """A row's bits are the same alone and among others of its kind of step, as in the other tensor-core kernels."""
     N, K = 512, 1024

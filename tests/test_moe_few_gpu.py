@@ -91,6 +91,17 @@ def test_layer(ops, weights, T, E, k, H, I):
     close(call(ops, c, k, scoring="softmax_chosen", scale=1.3, out_dtype=BF16), y, bound)
 
 
+# widths at which a block of the grid has more than 16 and more than 32 rows of the down matrices, and each of its warps several
+# blocks of K of the chosen experts
+@pytest.mark.parametrize("weights", ["bfloat16", "e4m3"])
+@pytest.mark.parametrize("T,E,k,H,I", [(1, 8, 3, 5120, 1000), (5, 8, 2, 5120, 1048), (12, 8, 3, 5120, 1000), (3, 4, 2, 9008, 1200),
+                                       (16, 6, 3, 9000, 1000), (8, 6, 2, 7104, 1304)])
+def test_wide_layer(ops, weights, T, E, k, H, I):
+    c = layer(ops, T, E, H, I, weights, seed=T + H)
+    expert, weight, _ = ops.router_topk(c["h32"], c["router"], k, renormalize=True)
+    close(call(ops, c, k, renormalize=True), *plain(c, expert, weight, "output"))
+
+
 @pytest.mark.parametrize("T,H,I", [(1, 257, 130), (11, 1001, 74), (4, 17, 2)])
 def test_odd_widths_of_8_bit_weights(ops, T, H, I):
     c = layer(ops, T, 6, H, I, "e4m3", seed=H)
