@@ -825,3 +825,17 @@ SHARPI_API int sharpi_softcap(float* y, float cap, long long n, cudaStream_t str
     SHARPI_LAUNCH_PDL(softcap_kernel, (unsigned)((n + 255) / 256), 256, 0, stream, y, cap, n);
     return SHARPI_OK;
 }
+
+// `bytes` at p are zero when this returns, on no stream of the caller's: a capture under way neither records it nor is ended by it
+SHARPI_API int sharpi_zero_now(void* p, long long bytes) {
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    if (cudaThreadExchangeStreamCaptureMode(&mode) != cudaSuccess) return SHARPI_LAUNCH_FAILED;
+    cudaStream_t own;
+    bool ok = cudaStreamCreateWithFlags(&own, cudaStreamNonBlocking) == cudaSuccess;
+    if (ok) {
+        ok = cudaMemsetAsync(p, 0, (size_t)bytes, own) == cudaSuccess && cudaStreamSynchronize(own) == cudaSuccess;
+        cudaStreamDestroy(own);
+    }
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    return ok ? SHARPI_OK : SHARPI_LAUNCH_FAILED;
+}

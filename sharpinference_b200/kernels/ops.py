@@ -512,8 +512,14 @@ def status_word(device) -> torch.Tensor:
         device = torch.device(device)
         w = _status_words.get(device)
         if w is None:
-            w = torch.zeros(1, dtype=torch.int32, device=device)
-            _status_words[device] = w
+            if device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+                # zeroed beside the capture: as a part of the graph every replay would zero it, whatever a kernel has recorded
+                w = torch.empty(1, dtype=torch.int32, device=device)
+                with torch.cuda.device(device):
+                    check(kernel("sharpi_zero_now")(w.data_ptr(), 4), "sharpi_zero_now")
+            else:
+                w = torch.zeros(1, dtype=torch.int32, device=device)
+            w = _status_words.setdefault(device, w)
     return w
 
 

@@ -444,6 +444,28 @@ def test_in_a_graph_and_on_another_stream(ops):
     assert torch.equal(got, want)
 
 
+def test_the_first_call_of_a_process_captured(ops, monkeypatch):
+    """The status word that a captured call brings into being is zero at once and is no part of the graph: a replay does not take
+    back what a kernel has recorded."""
+    t = operands(ops, 3, 200, 300)
+    want = ops.fp8_dense(*t)
+    torch.cuda.synchronize()
+    monkeypatch.setattr(ops, "_status_words", {})
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = ops.fp8_dense(*t)
+    word = ops.status_word(DEV)
+    ops.check_status(DEV)
+    g.replay()
+    word.fill_(8)
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
+    with pytest.raises(ops.KernelError, match="code 8"):
+        ops.check_status(DEV)
+    ops.check_status(DEV)
+
+
 @pytest.mark.parametrize("split", [1, 2, 3, 5, 8])
 @pytest.mark.parametrize("M,N,K", [(1, 300, 1024), (37, 256, 1100), (128, 130, 1153), (200, 515, 2048)])
 def test_split_over_k(ops, split, M, N, K):
