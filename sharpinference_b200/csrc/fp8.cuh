@@ -13,8 +13,6 @@
 
 #include "common.cuh"
 
-#include <cuda_fp16.h>
-
 namespace fp8 {
 
 constexpr int BLOCK = 128;                            // elements along K (and, for weights, rows) that share a scale
@@ -34,14 +32,6 @@ __device__ __forceinline__ uint32_t pack4(float a, float b, float c, float d) {
     asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(b), "f"(a));
     asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(d), "f"(c));
     return (uint32_t)lo | ((uint32_t)hi << 16);
-}
-
-__device__ __forceinline__ float to_float(uint8_t q) {
-    uint32_t h2;
-    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h2) : "h"((uint16_t)q));
-    __half_raw h;
-    h.x = (unsigned short)(h2 & 0xffffu);
-    return __half2float(__half(h));
 }
 
 }  // namespace fp8

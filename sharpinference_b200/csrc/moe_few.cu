@@ -34,6 +34,8 @@
 #include "fp8.cuh"
 #include "mma_sync.cuh"
 
+#include <cuda_fp16.h>
+
 namespace {
 
 constexpr int MAX_T = 16, MAX_K = 32, MAX_E = 1024;
