@@ -14,7 +14,8 @@
 // multiply the scales of rows and weights into a ring in shared memory (a factor a row and weight tile), so the readers' loop
 // is loads from tensor memory and paired multiply-adds with one factor.  The registers go where the sums are (setmaxnreg: 2 x
 // 224 + 56).  4096 x 16384 x 5120: 330 us; sixteen readers with 64 sums each (104 registers, which spill) 356; with the operands
-// swapped (weight rows on the lanes, a factor a column) 650 to 920.
+// swapped (weight rows on the lanes, a factor a column) 650 to 920.  The walks spill 0 (store) and 4 bytes a thread (SwiGLU), the
+// clusters 104 and 12.
 //
 // Two grids.  Many tiles: one CTA an SM that walks tiles of all experts, those of one weight tile one after the other; copies
 // and MMAs of its next tile run while the last one's sums are written.  Few tiles: a cluster of S CTAs a tile, each with its

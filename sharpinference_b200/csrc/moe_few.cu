@@ -21,13 +21,15 @@
 //
 // bfloat16 weights: mma.sync m16n8k16.  act is two bfloat16, its rounding and what that left (together within 2^-16 of its
 // value), multiplied one after the other into the same sums.  With the first alone (2^-8) a layer in bfloat16 is off by 1.4 times
-// its own rounding; the second costs 27.8 us for 27.0 (one token, 8 of 128 experts, 2048 x 768) and 163 for 145 (16 tokens).
+// its own rounding; the second costs 27.8 us for 27.0 (one token, 8 of 128 experts, 2048 x 768) and 163 for 145 (16 tokens; the
+// selection of sums brings 2 more).
 //
 // e4m3 weights with a scale for 128 x 128 (fp8.cuh): an e4m3 value is a float16 one (cvt, two an instruction), and the MMA is
 // m16n8k16 on float16.  (mma.sync on e4m3 is no instruction of this GPU's: it converts both operands for every tile, 1000
 // instructions a step of 4 KB where this takes 250.)  The activations are float16 times a power of two s for 128 neighbours such
-// that |x / s| < 2^15: of h's eight bits none is lost down to 2^-32 of its block's largest value, act is off by 2^-11 of its
-// value.  A block's 128 products are added in float32, then scaled and added.  Infinities and NaN make a block's scale NaN.
+// that the largest |x / s| is 2^14 to 2^15: of h's eight bits none is lost down to 2^-31 of its block's largest value; act is off by
+// 2^-11 of its value, or, below 2^-28 of its block's largest, by 2^-39 of that.  A block's 128 products are added in float32, then
+// scaled and added.  Infinities and NaN make a block's scale NaN.  9 to 16 tokens spill (202 bytes a thread; bfloat16 18, else none).
 //
 // The barrier needs all CTAs on the GPU at once: the launch is cooperative.  Its counters lie in the call's own workspace and
 // are set to zero by the router kernel.  The wait is bounded; on a timeout the kernel sets *status and returns.

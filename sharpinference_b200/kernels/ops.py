@@ -2271,7 +2271,8 @@ def fp8_dense(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: 
               out: Optional[torch.Tensor] = None, out_dtype: torch.dtype = torch.float32, accumulate: bool = False) -> torch.Tensor:
     """``a . w^T (+ bias)`` of block-scaled 8-bit operands: ``a`` e4m3 ``[M, K]`` with ``a_scale [blocks of K, M]`` (from
     :func:`fp8_rows`), ``w`` e4m3 ``[N, K]`` with ``w_scale [blocks of N, blocks of K]`` (from :func:`fp8_weight`).  Sums are
-    float32; ``[M, N]`` float32 or bfloat16, or added into float32 ``out`` when ``accumulate``."""
+    float32; ``[M, N]`` float32 or bfloat16, or added into float32 ``out`` when ``accumulate``.  Into how many parts K is cut goes by
+    the sizes of the call, so a row's result among few rows and among many may differ by float32 rounding (all products here)."""
     if w.dim() != 2:
         raise KernelError(f"a dense product needs w [N, K], found {tuple(w.shape)}")
     return _fp8_product(a, a_scale, w, w_scale, None, bias=bias, out=out, out_dtype=out_dtype, accumulate=accumulate)
@@ -2340,17 +2341,20 @@ def moe_few(h: torch.Tensor, router_weight: torch.Tensor, gate_up: torch.Tensor,
             renormalize: bool = False, scale: float = 1.0, weights_on: str = "output", add: Optional[torch.Tensor] = None,
             out: Optional[torch.Tensor] = None, out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """A whole mixture layer for up to 16 tokens in two kernels: router, choice of ``k`` gated experts a token, both products and
-    the weighted sum; ``[T, H]`` float32 or bfloat16.
+    the weighted sum; ``[T, H]`` float32 or bfloat16.  Against the chain of :func:`router_topk`, :func:`moe_sort`, two grouped
+    products and :func:`moe_combine` it takes 0.4 to 0.7 of the time for one token and is ahead up to 4 to 8; from 12 tokens on the
+    chain is, but for small layers (experts of 2048 x 768 or 4096 x 1024 in bfloat16).
 
     ``h`` bfloat16 ``[T, H]``; ``h32`` (float32, optional) are the unrounded activations, which the router reads instead.
     Choice and weights (``router_weight``, ``correction``, ``bias``, ``scoring``, ``renormalize``, ``scale``) as in
-    :func:`router_topk`; a NaN among a token's logits makes its output NaN.  ``gate_up`` ``[E, 2 I, H]`` holds gate rows then up
+    :func:`router_topk`; a NaN among a token's logits makes its output NaN.  What is not finite in an expert's weights touches the
+    tokens that chose it alone.  ``gate_up`` ``[E, 2 I, H]`` holds gate rows then up
     rows, ``down`` is ``[E, H, I]``: both bfloat16 with ``H`` and ``I`` multiples of 8, or both e4m3 with the scales of
     :func:`fp8_weight` and an even ``I``.  ``weights_on``: a weight multiplies its expert's ``"input"`` (before the nonlinearity) or
     ``"output"``.  ``add`` float32 ``[T, H]`` is added (a shared expert's output; ``out`` may be it).
 
     Between the products ``silu(g) * u`` is two bfloat16 (2^-16 of its value), or (e4m3 weights) float16 times a power of two for
-    128 neighbours (2^-11); sums are float32.  The order in which a token's terms are added goes by the experts that the whole call reaches."""
+    128 neighbours (2^-11 of its value, or 2^-39 of the largest of them where that is more); sums are float32.  The order in which a token's terms are added goes by the experts that the whole call reaches."""
     _need(h, "h", torch.bfloat16)
     _need(router_weight, "router_weight", torch.float32)
     if h.dim() != 2 or router_weight.dim() != 2 or gate_up.dim() != 3 or down.dim() != 3:
